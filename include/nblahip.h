@@ -40,7 +40,9 @@ extern "C" {
 
 #define NBLAHIP_EXPORT __attribute__((visibility("default")))
 
-enum nblahip_dtype { NBLAHIP_F32 = 0, NBLAHIP_F16 = 1 };
+/* NBLAHIP_BF16: the transformer-block functions only (RMSNormalization, the
+ * residual step, 8-bit checkpoints); the others refuse it with NBLAHIP_EINVAL. */
+enum nblahip_dtype { NBLAHIP_F32 = 0, NBLAHIP_F16 = 1, NBLAHIP_BF16 = 2 };
 
 enum nblahip_status {
   NBLAHIP_OK = 0,
@@ -414,6 +416,132 @@ NBLAHIP_EXPORT int nblahip_in_cl_bwd(const void *x, const void *dy,
                                      int64_t channels, int bc_gamma, int bc_beta,
                                      float eps, int dtype, void *workspace,
                                      size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------
+ * Transformer blocks.  No counterpart in the reference: the norms that stand
+ * before and after a block of a transformer, fused with what stands between
+ * them, and 8-bit copies of their inputs for the backward pass.
+ *
+ * Tensors are [rows, cols], contiguous, a row per token; dtype is NBLAHIP_F32,
+ * NBLAHIP_F16 or NBLAHIP_BF16.  Any number of rows and columns (cols below
+ * 2^31, fewer than 2^46 elements) at element alignment.  Parameters, shared
+ * gates, statistics and their gradients are float32, all arithmetic too; each
+ * output is rounded once.  The norms are over the columns:
+ *   RMS   : v / sqrt(mean(v^2) + eps) * gamma               (saved: mean square)
+ *   LAYER : (v - mean) / sqrt(var + eps) * gamma + beta     (saved: mean, biased var)
+ * A NULL gamma / beta stands for 1 / 0; RMS has no beta.
+ *
+ * Aliasing: an output tensor may be an input tensor of its shape and dtype
+ * itself (h may be res: the stream is updated in place); other overlaps of an
+ * output with an input, a parameter, a saved statistic, the workspace or
+ * another output are refused with NBLAHIP_EALIAS.
+ * ---------------------------------------------------------------------- */
+
+/* 8-bit copies of activations.  Each run of 32 columns of a row (the last may
+ * be shorter) shares a scale 2^(code - 127), one byte: the least power of two,
+ * not below 2^-120, at which the run's largest magnitude fits: rounds to 127 or
+ * less (INT8: two's complement), is 448 or less (E4M3: 4 exponent and 3
+ * mantissa bits, finite only).  Codes are rounded to nearest, ties to even.  A
+ * run that holds an infinity or NaN has code 255 and reads back as NaN.  A copy
+ * of rows x cols is rows*cols bytes of codes and rows*ceil(cols/32) of scales. */
+enum nblahip_act8_format { NBLAHIP_ACT8_NONE = 0, NBLAHIP_ACT8_INT8 = 1, NBLAHIP_ACT8_E4M3 = 2 };
+
+NBLAHIP_EXPORT int64_t nblahip_act8_scales_per_row(int64_t cols);
+NBLAHIP_EXPORT int nblahip_act8_pack(const void *x, void *codes, uint8_t *scales,
+                                     int64_t rows, int64_t cols, int format,
+                                     int dtype, void *stream);
+/* x = code * scale, rounded to dtype. */
+NBLAHIP_EXPORT int nblahip_act8_unpack(const void *codes, const uint8_t *scales,
+                                       void *x, int64_t rows, int64_t cols,
+                                       int format, int dtype, void *stream);
+
+/* RMSNormalization.  ms[rows] (the mean squares) is always written. */
+NBLAHIP_EXPORT int nblahip_rms_fwd(const void *x, const float *gamma, void *y,
+                                   float *ms, int64_t rows, int64_t cols,
+                                   float eps, int dtype, void *stream);
+NBLAHIP_EXPORT size_t nblahip_rms_bwd_workspace_bytes(int64_t rows, int64_t cols,
+                                                      int dtype);
+/* x_format NONE: x is the input (dtype); else its 8-bit copy with x_scale.  dx
+ * and dgamma may be NULL (not propagated).  No rows: dgamma is zero. */
+NBLAHIP_EXPORT int nblahip_rms_bwd(const void *x, const uint8_t *x_scale,
+                                   int x_format, const void *dy,
+                                   const float *gamma, const float *ms, void *dx,
+                                   float *dgamma, int accum_dx, int accum_dgamma,
+                                   int64_t rows, int64_t cols, float eps,
+                                   int dtype, void *workspace,
+                                   size_t workspace_bytes, void *stream);
+
+/* LayerNormalization backward (one-output form) from an 8-bit copy of x;
+ * mean / var are those nblahip_ln_fwd wrote.  dtype: of dy and dx. */
+NBLAHIP_EXPORT size_t nblahip_ln_bwd_act8_workspace_bytes(int64_t outer,
+                                                          int64_t reduce,
+                                                          int dtype);
+NBLAHIP_EXPORT int nblahip_ln_bwd_act8(const void *x8, const uint8_t *x_scale,
+                                       int x_format, const void *dy,
+                                       const float *gamma, const float *mean,
+                                       const float *var, void *dx, float *dgamma,
+                                       float *dbeta, int accum_dx,
+                                       int accum_dgamma, int accum_dbeta,
+                                       int64_t outer, int64_t reduce, float eps,
+                                       int dtype, void *workspace,
+                                       size_t workspace_bytes, void *stream);
+
+/* The step between two blocks of a residual stream.  x is the output of the
+ * block before, res the stream:
+ *   u = post ? norm(x; gamma_post, beta_post) : x
+ *   h = res_scale * res + branch_scale * gate * u       (res NULL: no residual)
+ *   y = norm(h; gamma_pre, beta_pre)                    (pre != 0)
+ * h is the stream after the step and y the next block's input; y is computed
+ * from h before h's rounding.  At least one of post and pre.
+ * gate_kind: NONE; ROWS: float32 [gate_rows, cols], gate row g scales rows
+ * g*rows/gate_rows onward (1: a learned scale per channel; a row per sample: the
+ * gate of a conditioned block), gate_rows divides rows; FULL: [rows, cols] of
+ * dtype.  x8 / h8 with their scales (each pair may be NULL) receive the 8-bit
+ * copies of x and of h as stored that nblahip_act8_pack would make. */
+enum nblahip_norm_kind { NBLAHIP_NORM_RMS = 0, NBLAHIP_NORM_LAYER = 1 };
+enum nblahip_gate_kind { NBLAHIP_GATE_NONE = 0, NBLAHIP_GATE_ROWS = 1, NBLAHIP_GATE_FULL = 2 };
+
+NBLAHIP_EXPORT int nblahip_resnorm_fwd(
+    const void *x, const void *res, const void *gate, int gate_kind,
+    int64_t gate_rows, const float *gamma_post, const float *beta_post,
+    const float *gamma_pre, const float *beta_pre, void *h, void *y,
+    float *mean_post, float *var_post, float *mean_pre, float *var_pre,
+    void *x8, uint8_t *x8_scale, void *h8, uint8_t *h8_scale, int format8,
+    int64_t rows, int64_t cols, float res_scale, float branch_scale, float eps,
+    int norm, int post, int pre, int dtype, void *stream);
+
+NBLAHIP_EXPORT size_t nblahip_resnorm_bwd_workspace_bytes(
+    int64_t rows, int64_t cols, int gate_kind, int64_t gate_rows, int norm,
+    int post, int pre, int dtype);
+
+/* Bits of `accum`: add onto the gradient instead of overwriting it. */
+enum nblahip_accum {
+  NBLAHIP_ACCUM_DX = 1,
+  NBLAHIP_ACCUM_DRES = 2,
+  NBLAHIP_ACCUM_DGATE = 4,
+  NBLAHIP_ACCUM_DGAMMA_POST = 8,
+  NBLAHIP_ACCUM_DBETA_POST = 16,
+  NBLAHIP_ACCUM_DGAMMA_PRE = 32,
+  NBLAHIP_ACCUM_DBETA_PRE = 64
+};
+
+/* x and h are the tensors of the forward (kept_format NONE) or both their 8-bit
+ * copies; x is read if post or gated, h if pre (else NULL).  dh: the gradient
+ * of h from the stream's later readers (NULL: none; required without pre); dy:
+ * of y (pre).  With t = dh + norm'(dy):  dres = res_scale * t,
+ * dgate = branch_scale * t * u summed over the rows a gate row serves,
+ * dx = norm'(branch_scale * gate * t).  Every gradient may be NULL. */
+NBLAHIP_EXPORT int nblahip_resnorm_bwd(
+    const void *x, const uint8_t *x_scale, const void *h, const uint8_t *h_scale,
+    int kept_format, const void *dh, const void *dy, const void *gate,
+    int gate_kind, int64_t gate_rows, const float *gamma_post,
+    const float *beta_post, const float *gamma_pre, const float *mean_post,
+    const float *var_post, const float *mean_pre, const float *var_pre, void *dx,
+    void *dres, void *dgate, float *dgamma_post, float *dbeta_post,
+    float *dgamma_pre, float *dbeta_pre, unsigned accum, int64_t rows,
+    int64_t cols, float res_scale, float branch_scale, float eps, int norm,
+    int post, int pre, int dtype, void *workspace, size_t workspace_bytes,
+    void *stream);
 
 /* ------------------------------------------------------------------------
  * Runtime shims used by the backend's array class and singleton so that host

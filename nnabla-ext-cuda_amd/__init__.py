@@ -8,6 +8,7 @@ library has not been built.
 """
 from __future__ import annotations
 
+import collections
 import ctypes
 import os
 
@@ -16,7 +17,7 @@ LIB_PATH = os.path.join(_HERE, "lib", "libnblahip.so")
 HOST_LIB_PATH = os.path.join(_HERE, "lib", "libnnabla_hip.so")
 CSRC = os.path.join(_HERE, "csrc")
 
-F32, F16 = 0, 1
+F32, F16, BF16 = 0, 1, 2
 
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -69,6 +70,22 @@ SIGNATURES = {
                                                                 _sz, _c_void_p]),
     "nblahip_in_cl_bwd": (_int, [_c_void_p] * 10 + [_int] * 3 + [_i64] * 3 + [_int, _int, _f, _int,
                                                                       _c_void_p, _sz, _c_void_p]),
+    "nblahip_act8_scales_per_row": (_i64, [_i64]),
+    "nblahip_act8_pack": (_int, [_c_void_p] * 3 + [_i64] * 2 + [_int, _int, _c_void_p]),
+    "nblahip_act8_unpack": (_int, [_c_void_p] * 3 + [_i64] * 2 + [_int, _int, _c_void_p]),
+    "nblahip_rms_fwd": (_int, [_c_void_p] * 4 + [_i64] * 2 + [_f, _int, _c_void_p]),
+    "nblahip_rms_bwd_workspace_bytes": (_sz, [_i64] * 2 + [_int]),
+    "nblahip_rms_bwd": (_int, [_c_void_p] * 2 + [_int] + [_c_void_p] * 5 + [_int] * 2 + [_i64] * 2 +
+                        [_f, _int, _c_void_p, _sz, _c_void_p]),
+    "nblahip_ln_bwd_act8_workspace_bytes": (_sz, [_i64] * 2 + [_int]),
+    "nblahip_ln_bwd_act8": (_int, [_c_void_p] * 2 + [_int] + [_c_void_p] * 7 + [_int] * 3 +
+                            [_i64] * 2 + [_f, _int, _c_void_p, _sz, _c_void_p]),
+    "nblahip_resnorm_fwd": (_int, [_c_void_p] * 3 + [_int, _i64] + [_c_void_p] * 14 + [_int] +
+                            [_i64] * 2 + [_f] * 3 + [_int] * 4 + [_c_void_p]),
+    "nblahip_resnorm_bwd_workspace_bytes": (_sz, [_i64] * 2 + [_int, _i64] + [_int] * 4),
+    "nblahip_resnorm_bwd": (_int, [_c_void_p] * 4 + [_int] + [_c_void_p] * 3 + [_int, _i64] +
+                            [_c_void_p] * 14 + [ctypes.c_uint] + [_i64] * 2 + [_f] * 3 + [_int] * 4 +
+                            [_c_void_p, _sz, _c_void_p]),
     "nblahip_device_count": (_int, [ctypes.POINTER(_int)]),
     "nblahip_set_device": (_int, [_int]),
     "nblahip_get_device": (_int, [ctypes.POINTER(_int)]),
@@ -581,3 +598,342 @@ def permute(x, perm, out=None, accum=False):
     check(lib().nblahip_permute(_ptr(x), _ptr(out), nd, shape, pm, int(accum), _dtype_code(x),
                                 _stream()))
     return out
+
+
+# ---------------------------------------------------------------------------
+# Transformer blocks: RMSNormalization, the residual step, 8-bit copies.  Rows
+# are `outer` runs of x.numel() // outer columns, as for ln_forward; float32,
+# float16 or bfloat16.
+# ---------------------------------------------------------------------------
+NORMS = {"rms": 0, "layer": 1}
+ACT8_FORMATS = {"int8": 1, "e4m3": 2}
+_ACCUM_BITS = (1, 2, 4, 8, 16, 32, 64)
+
+# 8-bit copy of a tensor: codes (int8 or float8_e4m3fn, the tensor's shape) and
+# scales (uint8 exponent codes, [rows, ceil(cols / 32)]).
+Act8 = collections.namedtuple("Act8", "codes scales")
+# stats = (mean_post, var_post, mean_pre, var_pre), None where there is none; x8
+# and h8: 8-bit copies for the backward (checkpoint), of what it will read.
+ResNorm = collections.namedtuple("ResNorm", "h y stats x8 h8")
+ResNormGrads = collections.namedtuple(
+    "ResNormGrads", "dx dres dgate dgamma_post dbeta_post dgamma_pre dbeta_pre")
+
+_token_dtypes = {}
+
+
+def _token_dtype(t):
+    if not _token_dtypes:
+        import torch
+        _token_dtypes.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    code = _token_dtypes.get(t)
+    if code is None:
+        raise TypeError(f"unsupported activation dtype {t}")
+    return code
+
+
+def _act8_format(a):
+    import torch
+    if a.codes.dtype == torch.int8:
+        return ACT8_FORMATS["int8"]
+    if a.codes.dtype == torch.float8_e4m3fn:
+        return ACT8_FORMATS["e4m3"]
+    raise TypeError(f"8-bit codes must be int8 or float8_e4m3fn, not {a.codes.dtype}")
+
+
+class _On:
+    """Current device = the tensors' device, and its current stream, for one
+    call; every tensor must be contiguous and on that device."""
+    __slots__ = ("device", "guard")
+
+    def __init__(self, first, *rest):
+        import torch
+        self.device = d = first.device
+        if d.type != "cuda":
+            raise TypeError(f"tensors must be on a GPU, not on {d}")
+        for t in (first,) + rest:
+            if t is None:
+                continue
+            if t.device != d:
+                raise ValueError(f"tensors on {d} and on {t.device} in one call")
+            if not t.is_contiguous():
+                raise ValueError("tensors must be contiguous")
+        self.guard = None if d.index == torch.cuda.current_device() else torch.cuda.device(d)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return _stream()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _rows_cols(t, outer):
+    n = t.numel()
+    if outer < 0 or (outer == 0 and n) or (outer and n % outer):
+        raise ValueError(f"{n} elements are not {outer} rows")
+    if outer:
+        return outer, n // outer
+    return 0, t.shape[-1] if t.dim() else 0
+
+
+def _like(t, n, dtype, name):
+    if t is not None and (t.dtype != dtype or t.numel() != n):
+        raise ValueError(f"{name}: {t.numel()} elements of {t.dtype} where {n} of {dtype} are needed")
+    return t
+
+
+def _check_kept(k, name, rows, cols, dtype):
+    """A kept tensor (or its 8-bit copy) of rows x cols: (data, scales, format)."""
+    import torch
+    if k is None:
+        return None, None, 0
+    if isinstance(k, Act8):
+        _like(k.scales, rows * ((cols + 31) // 32), torch.uint8, name + ".scales")
+        if k.codes.numel() != rows * cols:
+            raise ValueError(f"{name}.codes: {k.codes.numel()} elements, not {rows} x {cols}")
+        return k.codes, k.scales, _act8_format(k)
+    _like(k, rows * cols, dtype, name)
+    return k, None, 0
+
+
+def act8_pack(x, outer, format="int8"):
+    """8-bit copy of x: Act8(codes like x, scales [outer, ceil(cols / 32)])."""
+    import torch
+    rows, cols = _rows_cols(x, outer)
+    f = ACT8_FORMATS[format]
+    with _On(x) as st:
+        codes = torch.empty(x.shape, dtype=torch.int8 if f == 1 else torch.float8_e4m3fn, device=x.device)
+        scales = torch.empty((rows, (cols + 31) // 32), dtype=torch.uint8, device=x.device)
+        check(lib().nblahip_act8_pack(_ptr(x), _ptr(codes), _ptr(scales), rows, cols, f,
+                                      _token_dtype(x.dtype), st))
+    return Act8(codes, scales)
+
+
+def act8_unpack(a, outer, dtype, out=None):
+    """The values an 8-bit copy stands for, rounded to dtype."""
+    import torch
+    rows, cols = _rows_cols(a.codes, outer)
+    codes, scales, f = _check_kept(a, "a", rows, cols, dtype)
+    with _On(codes, scales, out) as st:
+        if out is None:
+            out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+        _like(out, rows * cols, dtype, "out")
+        check(lib().nblahip_act8_unpack(_ptr(codes), _ptr(scales), _ptr(out), rows, cols, f,
+                                        _token_dtype(dtype), st))
+    return out
+
+
+def rms_forward(x, gamma, outer, eps=1e-5, y=None):
+    """RMSNormalization: y, ms (the rows' mean squares).  gamma may be None."""
+    import torch
+    rows, cols = _rows_cols(x, outer)
+    dt = _token_dtype(x.dtype)
+    with _On(x, gamma, y) as st:
+        _like(gamma, cols, torch.float32, "gamma")
+        y = torch.empty_like(x) if y is None else _like(y, rows * cols, x.dtype, "y")
+        ms = torch.empty(rows, dtype=torch.float32, device=x.device)
+        check(lib().nblahip_rms_fwd(_ptr(x), _ptr(gamma), _ptr(y), _ptr(ms), rows, cols, eps, dt, st))
+    return y, ms
+
+
+def rms_backward(x, dy, gamma, ms, outer, eps=1e-5, dx=None, dgamma=None, accum=(False, False),
+                 need=(True, True), ws=None):
+    """dx, dgamma of RMSNormalization; x is the forward's input or its 8-bit copy
+    (Act8).  need / accum = (dx, dgamma)."""
+    import torch
+    rows, cols = _rows_cols(dy, outer)
+    dt = _token_dtype(dy.dtype)
+    xd, xs, f = _check_kept(x, "x", rows, cols, dy.dtype)
+    with _On(dy, xd, xs, gamma, ms, dx, dgamma, ws) as st:
+        _like(gamma, cols, torch.float32, "gamma")
+        _like(ms, rows, torch.float32, "ms")
+        dx = None if not need[0] else torch.empty_like(dy) if dx is None else _like(
+            dx, rows * cols, dy.dtype, "dx")
+        dgamma = None if not need[1] else torch.empty(
+            cols, dtype=torch.float32, device=dy.device) if dgamma is None else _like(
+                dgamma, cols, torch.float32, "dgamma")
+        if ws is None:
+            ws = _workspace(lib().nblahip_rms_bwd_workspace_bytes(rows, cols, dt), dy.device)
+        check(lib().nblahip_rms_bwd(_ptr(xd), _ptr(xs), f, _ptr(dy), _ptr(gamma), _ptr(ms), _ptr(dx),
+                                    _ptr(dgamma), int(accum[0]), int(accum[1]), rows, cols, eps, dt,
+                                    _ptr(ws), ws.numel(), st))
+    return dx, dgamma
+
+
+def ln_backward_act8(x8, dy, gamma, mean, var, outer, eps=1e-5, dx=None, dgamma=None, dbeta=None,
+                     accum=(False, False, False), need=(True, True, True), ws=None):
+    """ln_backward (one-output form) from the 8-bit copy of the forward's input."""
+    import torch
+    if not isinstance(x8, Act8):
+        raise TypeError("x8 must be an Act8 (act8_pack)")
+    rows, cols = _rows_cols(dy, outer)
+    dt = _token_dtype(dy.dtype)
+    xd, xs, f = _check_kept(x8, "x8", rows, cols, dy.dtype)
+    with _On(dy, xd, xs, gamma, mean, var, dx, dgamma, dbeta, ws) as st:
+        _like(gamma, cols, torch.float32, "gamma")
+        _like(mean, rows, torch.float32, "mean")
+        _like(var, rows, torch.float32, "var")
+        dx = None if not need[0] else torch.empty_like(dy) if dx is None else _like(
+            dx, rows * cols, dy.dtype, "dx")
+        par = [None if not need[i] else torch.empty(cols, dtype=torch.float32, device=dy.device)
+               if t is None else _like(t, cols, torch.float32, n)
+               for i, t, n in ((1, dgamma, "dgamma"), (2, dbeta, "dbeta"))]
+        if ws is None:
+            ws = _workspace(lib().nblahip_ln_bwd_act8_workspace_bytes(rows, cols, dt), dy.device)
+        check(lib().nblahip_ln_bwd_act8(_ptr(xd), _ptr(xs), f, _ptr(dy), _ptr(gamma), _ptr(mean),
+                                        _ptr(var), _ptr(dx), _ptr(par[0]), _ptr(par[1]),
+                                        int(accum[0]), int(accum[1]), int(accum[2]), rows, cols, eps,
+                                        dt, _ptr(ws), ws.numel(), st))
+    return dx, par[0], par[1]
+
+
+def _gate_args(gate, rows, cols, dtype):
+    """(kind, gate rows): an element each in the activations' dtype, or float32
+    rows [G, cols] ([cols]: one) that each serve rows / G tokens."""
+    import torch
+    if gate is None:
+        return 0, 0
+    n = gate.numel()
+    if gate.dtype == dtype and n == rows * cols and not (dtype == torch.float32 and rows == 1):
+        return 2, 0
+    if gate.dtype != torch.float32:
+        raise TypeError(f"gate: {tuple(gate.shape)} of {gate.dtype} for {rows} x {cols} of {dtype}; a "
+                        "gate of fewer rows is float32")
+    g = n // cols if cols else 0
+    if g == 0 or n != g * cols or rows % g:
+        raise ValueError(f"gate: {n} elements are no rows of {cols} that divide {rows}")
+    return 1, g
+
+
+def _step_params(cols, post, pre, norm, gamma_post, beta_post, gamma_pre, beta_pre):
+    import torch
+    if not (post or pre):
+        raise ValueError("a step has the norm after the block (post), the one before the next (pre) "
+                         "or both")
+    for p, name, on in ((gamma_post, "gamma_post", post), (beta_post, "beta_post", post),
+                        (gamma_pre, "gamma_pre", pre), (beta_pre, "beta_pre", pre)):
+        if p is None:
+            continue
+        if not on:
+            raise ValueError(f"{name} without its norm")
+        if name.startswith("beta") and norm == "rms":
+            raise ValueError(f"{name}: RMS normalization has no beta")
+        _like(p, cols, torch.float32, name)
+
+
+def resnorm_forward(x, res, outer, gate=None, gamma_post=None, beta_post=None, gamma_pre=None,
+                    beta_pre=None, norm="rms", post=True, pre=True, res_scale=1.0, branch_scale=1.0,
+                    eps=1e-5, checkpoint=None, h=None, y=None):
+    """The step between two blocks of a residual stream:
+        u = norm(x; gamma_post, beta_post) if post else x
+        h = res_scale * res + branch_scale * gate * u
+        y = norm(h; gamma_pre, beta_pre) if pre else None
+    gate: None, float32 [G, cols] (G divides outer) or a tensor like x.
+    checkpoint "int8" / "e4m3": also 8-bit copies x8, h8 of what the backward
+    reads.  h may be res, y may be x (in place).  Returns ResNorm."""
+    import torch
+    rows, cols = _rows_cols(x, outer)
+    dt, kind = _token_dtype(x.dtype), NORMS[norm]
+    layer = kind == 1
+    with _On(x, res, gate, gamma_post, beta_post, gamma_pre, beta_pre, h, y) as st:
+        _like(res, rows * cols, x.dtype, "res")
+        _step_params(cols, post, pre, norm, gamma_post, beta_post, gamma_pre, beta_pre)
+        gk, gr = _gate_args(gate, rows, cols, x.dtype)
+        h = torch.empty_like(x) if h is None else _like(h, rows * cols, x.dtype, "h")
+        if pre:
+            y = torch.empty_like(x) if y is None else _like(y, rows * cols, x.dtype, "y")
+        else:
+            y = None
+        # the statistics in one allocation
+        each = torch.empty(((int(post) + int(pre)) * (1 + kind), rows), dtype=torch.float32,
+                           device=x.device).unbind(0)
+        it = iter(each)
+        stats = [next(it) if on and (layer or k) else None
+                 for on in (post, pre) for k in (0, 1)]
+        x8 = h8 = None
+        f = 0
+        if checkpoint is not None:
+            f = ACT8_FORMATS[checkpoint]
+            qd = torch.int8 if f == 1 else torch.float8_e4m3fn
+
+            def copy():
+                return Act8(torch.empty(x.shape, dtype=qd, device=x.device),
+                            torch.empty((rows, (cols + 31) // 32), dtype=torch.uint8, device=x.device))
+            x8 = copy() if post or gk else None
+            h8 = copy() if pre else None
+        check(lib().nblahip_resnorm_fwd(
+            _ptr(x), _ptr(res), _ptr(gate), gk, gr, _ptr(gamma_post), _ptr(beta_post), _ptr(gamma_pre),
+            _ptr(beta_pre), _ptr(h), _ptr(y), _ptr(stats[0]), _ptr(stats[1]), _ptr(stats[2]),
+            _ptr(stats[3]), _ptr(x8 and x8.codes), _ptr(x8 and x8.scales), _ptr(h8 and h8.codes),
+            _ptr(h8 and h8.scales), f, rows, cols, res_scale, branch_scale, eps, kind, int(post),
+            int(pre), dt, st))
+    return ResNorm(h, y, tuple(stats), x8, h8)
+
+
+def resnorm_backward(x, h, dh, dy, stats, outer, gate=None, gamma_post=None, beta_post=None,
+                     gamma_pre=None, beta_pre=None, norm="rms", post=True, pre=True, res_scale=1.0,
+                     branch_scale=1.0, eps=1e-5, has_res=True, need=(True,) * 7, accum=(False,) * 7,
+                     out=None, ws=None):
+    """Gradients of resnorm_forward.  x, h: its tensors, or their 8-bit copies
+    (both); dh: gradient of h from its later readers (None: none), dy: of y.
+    need / accum / out follow ResNormGrads' fields; what does not exist (dres
+    without a residual, dgate without a gate, parameters of an absent norm, beta
+    of RMS) is None."""
+    import torch
+    lead = dh if dh is not None else dy
+    if lead is None:
+        raise ValueError("dh or dy is needed")
+    rows, cols = _rows_cols(lead, outer)
+    act, dt, kind = lead.dtype, _token_dtype(lead.dtype), NORMS[norm]
+    layer = kind == 1
+    gk, gr = _gate_args(gate, rows, cols, act)
+    if not (post or gk):
+        x = None
+    if not pre:
+        h = dy = None
+    xd, xs, xf = _check_kept(x, "x", rows, cols, act)
+    hd, hs, hf = _check_kept(h, "h", rows, cols, act)
+    if x is not None and h is not None and xf != hf:
+        raise TypeError("x and h must be kept in the same form")
+    out = ResNormGrads(*([None] * 7)) if out is None else out
+    with _On(lead, dh, dy, xd, xs, hd, hs, gate, gamma_post, beta_post, gamma_pre, beta_pre, *stats,
+             *out, ws) as st:
+        _step_params(cols, post, pre, norm, gamma_post, beta_post, gamma_pre, beta_pre)
+        _like(dh, rows * cols, act, "dh")
+        _like(dy, rows * cols, act, "dy")
+        for s, name in zip(stats, ("mean_post", "var_post", "mean_pre", "var_pre")):
+            _like(s, rows, torch.float32, name)
+        have = (True, has_res, gk != 0, post, post and layer, pre, pre and layer)
+        f32 = torch.float32
+        shapes = ((lead.shape, act), (lead.shape, act),
+                  (None if gate is None else gate.shape, act if gk == 2 else f32),
+                  ((cols,), f32), ((cols,), f32), ((cols,), f32), ((cols,), f32))
+        grads = []
+        mask = 0
+        for i in range(7):
+            t = None
+            if have[i] and need[i]:
+                shape, d = shapes[i]
+                t = out[i]
+                if t is None:
+                    t = torch.empty(shape, dtype=d, device=lead.device)
+                else:
+                    n = 1
+                    for k in shape:
+                        n *= k
+                    _like(t, n, d, ResNormGrads._fields[i])
+                if accum[i]:
+                    mask |= _ACCUM_BITS[i]
+            grads.append(t)
+        if ws is None:
+            ws = _workspace(lib().nblahip_resnorm_bwd_workspace_bytes(
+                rows, cols, gk, gr, kind, int(post), int(pre), dt), lead.device)
+        p = [_ptr(g) for g in grads]
+        check(lib().nblahip_resnorm_bwd(
+            _ptr(xd), _ptr(xs), _ptr(hd), _ptr(hs), xf or hf, _ptr(dh), _ptr(dy), _ptr(gate), gk, gr,
+            _ptr(gamma_post), _ptr(beta_post), _ptr(gamma_pre), _ptr(stats[0]), _ptr(stats[1]),
+            _ptr(stats[2]), _ptr(stats[3]), p[0], p[1], p[2], p[3], p[4], p[5], p[6], mask, rows, cols,
+            res_scale, branch_scale, eps, kind, int(post), int(pre), dt, _ptr(ws), ws.numel(), st))
+    return ResNormGrads(*grads)

@@ -1,0 +1,67 @@
+// The residual step and the row norms of transformer blocks: problem
+// description and launch functions (resnorm_host.hip plans, the units
+// resnorm_fwd_*.hip and resnorm_bwd_*.hip hold the kernels).
+#pragma once
+
+#include "launch.hpp"
+
+namespace nblahip {
+
+// One step of `rows` rows of `cols` columns:
+//   u = post ? norm(x; gamma_post, beta_post) : x
+//   h = res_scale * res + branch_scale * gate * u
+//   y = pre ? norm(h; gamma_pre, beta_pre) : none
+// RMSNormalization is the step with post alone, no residual and no gate.
+struct StepArgs {
+  const void *x = nullptr;       // block output; backward: as kept (storage type or 8 bits)
+  const void *res = nullptr;
+  const void *gate = nullptr;    // gate_kind 1: float [gate_rows, cols]; 2: storage type [rows, cols]
+  const float *gamma_post = nullptr, *beta_post = nullptr;
+  const float *gamma_pre = nullptr, *beta_pre = nullptr;
+  void *h = nullptr, *y = nullptr;                     // forward: out
+  float *mean_post = nullptr, *var_post = nullptr;     // forward: out; backward: in
+  float *mean_pre = nullptr, *var_pre = nullptr;
+  uint8_t *x8 = nullptr, *x8_scale = nullptr;          // forward: 8-bit copies out
+  uint8_t *h8 = nullptr, *h8_scale = nullptr;
+  // backward
+  const void *kept_h = nullptr;
+  const uint8_t *kept_x_scale = nullptr, *kept_h_scale = nullptr; // 8-bit copies' scales
+  const void *dh = nullptr, *dy = nullptr;
+  void *dx = nullptr, *dres = nullptr, *dgate = nullptr; // dgate: float for gate_kind 1
+  float *dgamma_post = nullptr, *dbeta_post = nullptr;
+  float *dgamma_pre = nullptr, *dbeta_pre = nullptr;
+  unsigned accum = 0;            // NBLAHIP_ACCUM_*
+  float *row_sums = nullptr;     // workspace, long rows: [rows][4]
+  float *part_pre = nullptr;     // workspace: [blocks][1 or 2][pitch]
+  float *part_post = nullptr;    // workspace: [chunks][1 or 2][pitch]
+  int64_t rows = 0, cols = 0;
+  int64_t pitch = 0;             // floats between rows of the partial sums
+  int64_t rows_per_gate = 1;
+  int64_t chunk_rows = 1, chunks_per_gate = 1, chunks = 1; // backward: runs of rows with one gate row
+  int64_t groups8 = 0;           // 8-bit groups per row
+  int gate_kind = 0;
+  int format8 = 0;
+  int grid = 1;                  // blocks launched (= rows of part_pre)
+  float res_scale = 1.f, branch_scale = 1.f, eps = 0.f;
+};
+
+// What selects a kernel.
+struct StepPlan {
+  int dtype = 0;
+  bool layer = false, post = false, pre = false;
+  bool kept8 = false;            // backward: x and h are 8-bit copies
+  int tpr = 0, nv = 0;           // threads per row, vectors per thread; 0: the kernels for long rows
+};
+
+// Rows a block works on at a time.
+inline int step_rows_per_block(int tpr) { return tpr < 256 ? 256 / tpr : 1; }
+inline int step_block(int tpr) { return tpr < 256 ? 256 : tpr; }
+
+int launch_step_fwd_f32(const StepPlan &pl, const StepArgs &a, hipStream_t st);
+int launch_step_fwd_f16(const StepPlan &pl, const StepArgs &a, hipStream_t st);
+int launch_step_fwd_bf16(const StepPlan &pl, const StepArgs &a, hipStream_t st);
+int launch_step_bwd_f32(const StepPlan &pl, const StepArgs &a, hipStream_t st);
+int launch_step_bwd_f16(const StepPlan &pl, const StepArgs &a, hipStream_t st);
+int launch_step_bwd_bf16(const StepPlan &pl, const StepArgs &a, hipStream_t st);
+
+} // namespace nblahip

@@ -1,0 +1,307 @@
+"""RMSNormalization and the residual step against the float64 oracle: types,
+norms, gates, sizes from one element to long rows, 8-bit copies, in-place
+calls, accumulation, graphs and streams."""
+import numpy as np
+import pytest
+import torch
+
+from _step import DTYPES, Step, close, f64
+from _util import load_package
+from oracle import step_ref as S
+
+K = load_package()
+pytestmark = pytest.mark.gpu
+
+# one element, less than a vector, odd, vector-sized, every layout's first and
+# last widths, rows too long for registers
+COLS = [1, 3, 8, 33, 100, 127, 128, 129, 256, 512, 513, 1000, 1024, 1027, 2048, 2560, 4096, 4100, 8192,
+        8193, 16384, 32768, 40001]
+
+
+def run(st, kept=None, need=(True,) * 7):
+    """Forward and backward of a Step, both checked."""
+    f = K.resnorm_forward(st.x, st.res, st.rows, checkpoint=kept, **st.args())
+    st.check_fwd(f)
+    if kept:
+        for t, c, used in ((st.x, f.x8, st.post or st.gate is not None), (f.h, f.h8, st.pre)):
+            assert (c is not None) == used
+            if used:
+                want = K.act8_pack(t, st.rows, kept)
+                assert torch.equal(c.scales, want.scales)
+                assert torch.equal(c.codes.view(torch.uint8), want.codes.view(torch.uint8))
+        x, h = f.x8, f.h8
+        xv, hv = (None if c is None else f64(K.act8_unpack(c, st.rows, torch.float32)) for c in (x, h))
+    else:
+        assert f.x8 is None and f.h8 is None
+        x, h = st.x, f.h
+        xv, hv = f64(x), f64(h)
+    g = K.resnorm_backward(x, h, st.dh, st.dy, f.stats, st.rows, has_res=st.res is not None,
+                           need=need, **st.args())
+    ref = st.oracle_bwd(xv, hv, f.stats)
+    st.check_grads(g, ref)
+    return f, g
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize("cols", COLS)
+def test_widths(cols, norm, dtype):
+    rows = 37 if cols < 9000 else 5
+    run(Step(rows, cols, dtype, norm, gate="channel", rs=0.8, bs=0.5))
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 16, 63, 64, 65, 255, 257, 1531, 5000])
+@pytest.mark.parametrize("cols", [24, 200, 1027, 2304])
+def test_row_counts(rows, cols):
+    run(Step(rows, cols, "bf16", "layer", gate="channel"))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize("post,pre", [(True, True), (True, False), (False, True)])
+@pytest.mark.parametrize("gate,samples", [("none", 1), ("channel", 1), ("sample", 6), ("sample", 48),
+                                          ("sample", 24), ("full", 1)])
+def test_every_form(gate, samples, post, pre, norm, dtype):
+    for cols, res in ((72, True), (1030, False), (20000 if dtype == "f32" else 33000, True)):
+        run(Step(48, cols, dtype, norm, post, pre, res, gate, samples, rs=1.25, bs=0.5))
+
+
+@pytest.mark.parametrize("kept", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize("post,pre,gate", [(True, True, "channel"), (True, False, "none"),
+                                           (False, True, "full"), (False, True, "none")])
+def test_from_eight_bits(post, pre, gate, norm, dtype, kept):
+    for rows, cols in ((33, 40), (20, 1000), (9, 4096), (3, 36000)):
+        run(Step(rows, cols, dtype, norm, post, pre, True, gate), kept)
+
+
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+def test_without_parameters(norm):
+    run(Step(40, 520, "f16", norm, gate="sample", samples=4, affine=False))
+    run(Step(5, 35000, "f16", norm, gate="full", affine=False))
+
+
+def test_no_gradient_from_later_readers():
+    for cols in (600, 33000):
+        st = Step(12, cols, "f16", "rms", gate="channel")
+        f = K.resnorm_forward(st.x, st.res, st.rows, **st.args())
+        g = K.resnorm_backward(st.x, f.h, None, st.dy, f.stats, st.rows, **st.args())
+        st.check_grads(g, st.oracle_bwd(f64(st.x), f64(f.h), f.stats, dh=None))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("shape", [(1, 1), (300, 64), (4096, 128), (70, 1000), (33, 4096), (3, 40001)])
+def test_rms(shape, dtype):
+    st = Step(*shape, dtype, pre=False, res=False)
+    x, dy = st.x, st.dh
+    y, ms = K.rms_forward(x, st.gp, shape[0], 1e-5)
+    ref = st.oracle_fwd()
+    close(y, *ref["h"], *shape, "y")
+    close(ms, ref["var_post"][:, 0], ref["var_post"][:, 0], *shape, "ms")
+    for kept in (None, "int8", "e4m3"):
+        xk = x if kept is None else K.act8_pack(x, shape[0], kept)
+        xv = f64(x if kept is None else K.act8_unpack(xk, shape[0], torch.float32))
+        dx, dg = K.rms_backward(xk, dy, st.gp, ms, shape[0], 1e-5)
+        ref = st.oracle_bwd(xv, None, (None, ms, None, None))
+        close(dx, *ref["dx"], *shape, "dx")
+        close(dg, *ref["dgamma_post"], *shape, "dgamma", column_sum=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("kept", ["int8", "e4m3"])
+def test_layer_norm_backward_from_eight_bits(kept, dtype):
+    """The forward is the framework's LayerNormalization."""
+    for shape in ((16, 96), (257, 1024), (9, 20002)):
+        st = Step(*shape, dtype, "layer", pre=False, res=False)
+        y, mean, var = K.ln_forward(st.x, st.bp, st.gp, shape[0])
+        x8 = K.act8_pack(st.x, shape[0], kept)
+        xv = f64(K.act8_unpack(x8, shape[0], torch.float32))
+        dx, dg, db = K.ln_backward_act8(x8, st.dh, st.gp, mean, var, shape[0])
+        ref = st.oracle_bwd(xv, None, (mean, var, None, None))
+        close(dx, *ref["dx"], *shape, "dx")
+        close(dg, *ref["dgamma_post"], *shape, "dgamma", column_sum=True)
+        close(db, *ref["dbeta_post"], *shape, "dbeta", column_sum=True)
+
+
+@pytest.mark.parametrize("cols", [200, 1030, 33000])
+def test_gradients_that_are_not_needed_and_accumulation(cols):
+    st = Step(24, cols, "f32", "layer", gate="sample", samples=4)
+    f, g = run(st)
+    for skip in range(7):
+        need = [i != skip for i in range(7)]
+        part = K.resnorm_backward(st.x, f.h, st.dh, st.dy, f.stats, st.rows, need=need, **st.args())
+        for i, name in enumerate(part._fields):
+            assert (part[i] is None) == (i == skip)
+            if part[i] is not None:
+                assert torch.equal(part[i], g[i]), name
+        alone = K.resnorm_backward(st.x, f.h, st.dh, st.dy, f.stats, st.rows,
+                                   need=[i == skip for i in range(7)], **st.args())
+        assert torch.equal(alone[skip], g[skip])
+    old = [torch.randn_like(t) for t in g]
+    out = K.ResNormGrads(*[t.clone() for t in old])
+    got = K.resnorm_backward(st.x, f.h, st.dh, st.dy, f.stats, st.rows, out=out, accum=(True,) * 7,
+                             **st.args())
+    for a, b, c, n in zip(got, g, old, got._fields):
+        # one more float32 addition, of values already rounded (or, summed here
+        # before the addition, not yet): two roundings of the larger of the two
+        assert ((a - (b + c)).abs() <= 2.0 ** -22 * (b.abs() + c.abs())).all(), n
+
+
+def test_in_place():
+    for cols in (520, 1030, 33000):
+        st = Step(20, cols, "f16", "layer", gate="full")
+        f, g = run(st)
+        x, res = st.x.clone(), st.res.clone()
+        p = K.resnorm_forward(x, res, st.rows, h=res, y=x, **st.args())
+        assert p.h is res and p.y is x
+        assert torch.equal(p.h, f.h) and torch.equal(p.y, f.y)
+        dh, dy, gate = st.dh.clone(), st.dy.clone(), st.gate.clone()
+        args = dict(st.args(), gate=gate)
+        out = K.ResNormGrads(dy, dh, gate, None, None, None, None)
+        q = K.resnorm_backward(st.x, f.h, dh, dy, f.stats, st.rows, out=out, **args)
+        for a, b in zip(q, g):
+            assert torch.equal(a, b)
+
+
+def test_same_bits_every_time():
+    st = Step(3000, 1040, "bf16", gate="channel")
+    f, g = run(st)
+    for _ in range(3):
+        f2 = K.resnorm_forward(st.x, st.res, st.rows, **st.args())
+        g2 = K.resnorm_backward(st.x, f.h, st.dh, st.dy, f.stats, st.rows, **st.args())
+        assert torch.equal(f.h, f2.h) and torch.equal(f.y, f2.y)
+        assert all(torch.equal(a, b) for a, b in zip(g, g2) if a is not None)
+
+
+def test_a_bad_row_stays_a_bad_row():
+    """An infinity or NaN reaches its own row (and the column sums), no other."""
+    for bad in (float("inf"), float("nan")):
+        st = Step(70, 264, "f32", "layer", gate="full")
+        f, g = run(st)
+        st.x[13, 100] = bad
+        f2 = K.resnorm_forward(st.x, st.res, st.rows, **st.args())
+        assert not torch.isfinite(f2.h[13]).any()
+        keep = [i for i in range(70) if i != 13]
+        assert torch.equal(f2.h[keep], f.h[keep]) and torch.equal(f2.y[keep], f.y[keep])
+        g2 = K.resnorm_backward(st.x, f2.h, st.dh, st.dy, f2.stats, st.rows, **st.args())
+        assert torch.equal(g2.dx[keep], g.dx[keep])
+        assert not torch.isfinite(g2.dgamma_post).any()
+
+
+def test_large_offset_rows():
+    """LayerNormalization of rows far from zero: the variance is about the mean."""
+    x = (torch.randn(9, 1000, generator=torch.Generator().manual_seed(1)) + 1000).cuda()
+    g = torch.ones(1000, device="cuda")
+    f = K.resnorm_forward(x, None, 9, gamma_post=g, norm="layer", pre=False)
+    xv = f64(x)
+    mean, var = S.moments(xv, "layer")
+    # the float32 mean is off by 2^-24 * 1000 at most per rounding: d = x - mean
+    # carries that, and y = d * rho with rho about 1
+    assert np.abs(f64(f.h) - (xv - mean) / np.sqrt(var + 1e-5)).max() < 16 * 2.0 ** -24 * 1000
+    assert np.abs(f64(f.stats[1]) - var[:, 0]).max() < 64 * 2.0 ** -24
+
+
+def test_only_the_outputs_are_written():
+    for cols in (100, 1030):
+        st = Step(6, cols, "f16", gate="channel")
+        n = 6 * cols
+        big = torch.full((n + 64,), 5.0, dtype=torch.float16, device="cuda")
+        f = K.resnorm_forward(st.x, st.res, 6, h=big[32:32 + n].view(6, cols), **st.args())
+        st.check_fwd(f)
+        assert (big[:32] == 5).all() and (big[32 + n:] == 5).all()
+        for off in (1, 2, 3):   # tensors at element alignment
+            x = torch.empty(n + 8, dtype=torch.float16, device="cuda")[off:off + n].view(6, cols)
+            x.copy_(st.x)
+            f2 = K.resnorm_forward(x, st.res, 6, **st.args())
+            assert torch.equal(f2.h, f.h) and torch.equal(f2.y, f.y)
+
+
+def test_no_rows():
+    z = torch.empty(0, 64, device="cuda")
+    f = K.resnorm_forward(z, z, 0)
+    assert f.h.shape == (0, 64) and f.y.shape == (0, 64)
+    y, ms = K.rms_forward(z, None, 0)
+    dx, dg = K.rms_backward(z, z, None, ms, 0)
+    assert (dg == 0).all() and dg.shape == (64,) and dx.shape == (0, 64)
+    a = K.act8_pack(z, 0)
+    assert K.act8_unpack(a, 0, torch.float32).shape == (0, 64)
+    g = K.resnorm_backward(z, z, z, z, f.stats, 0, gate=torch.ones(2, 64, device="cuda"))
+    assert (g.dgate == 0).all() and (g.dgamma_pre == 0).all() and (g.dgamma_post == 0).all()
+
+
+def test_a_run_of_blocks_trains_like_its_formula():
+    """Three residual steps with a linear block between them, forward and
+    backward from 8-bit copies and from the tensors, against float64."""
+    rows, cols, eps = 96, 160, 1e-5
+    gen = torch.Generator().manual_seed(3)
+    w = [(torch.randn(cols, cols, generator=gen) / cols ** 0.5) for _ in range(3)]
+    gp = [1 + 0.1 * torch.randn(cols, generator=gen) for _ in range(3)]
+    gn = [1 + 0.1 * torch.randn(cols, generator=gen) for _ in range(3)]
+    gate = [0.5 + 0.1 * torch.randn(1, cols, generator=gen) for _ in range(3)]
+    x0, r0, dy = (torch.randn(rows, cols, generator=gen) for _ in range(3))
+
+    leaves = [t.double().requires_grad_() for t in [x0, r0] + gp + gn + gate]
+    lx, lr, lgp, lgn, lg = leaves[0], leaves[1], leaves[2:5], leaves[5:8], leaves[8:11]
+
+    def rms(v, g):
+        return v / (v.pow(2).mean(1, keepdim=True) + eps).sqrt() * g
+    x, h = lx, lr
+    for i in range(3):
+        h = 0.9 * h + 0.5 * lg[i] * rms(x, lgp[i])
+        x = rms(h, lgn[i]) @ w[i].double()
+    (x * dy.double()).sum().backward()
+
+    dev = [t.cuda() for t in (x0, r0, dy)]
+    W, GP, GN, G = ([t.cuda() for t in l] for l in (w, gp, gn, gate))
+    for kept, tol in ((None, 1e-4), ("int8", 0.1)):
+        # float32 round-off over three steps stays below 1e-4 of the gradient's
+        # norm; int8 copies are off by 2^-7 of a group's largest magnitude (about
+        # three times its rms) at most, 0.012 of the rms on average, in each of
+        # the six norms: below a tenth of the norm
+        x, h, saved = dev[0], dev[1], []
+        for i in range(3):
+            kw = dict(gate=G[i], gamma_post=GP[i], gamma_pre=GN[i], res_scale=0.9, branch_scale=0.5)
+            f = K.resnorm_forward(x, h, rows, checkpoint=kept, **kw)
+            saved.append((kw, f.stats, f.x8 if kept else x, f.h8 if kept else f.h))
+            h, x = f.h, f.y @ W[i]
+        dx, dh, grads = dev[2], None, {}
+        for i in (2, 1, 0):
+            kw, stats, sx, sh = saved[i]
+            g = K.resnorm_backward(sx, sh, dh, dx @ W[i].t().contiguous(), stats, rows, **kw)
+            dh, dx = g.dres, g.dx
+            grads[i] = g
+        got = [dx, dh] + [grads[i].dgamma_post for i in range(3)] + [
+            grads[i].dgamma_pre for i in range(3)] + [grads[i].dgate for i in range(3)]
+        for a, b in zip(got, leaves):
+            d = a.double().cpu() - b.grad
+            assert d.norm() <= tol * b.grad.norm()
+
+
+def test_streams_and_graphs():
+    st = Step(128, 1040, "bf16", "layer", gate="channel")
+    f, g = run(st)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        f2 = K.resnorm_forward(st.x, st.res, st.rows, checkpoint="e4m3", **st.args())
+        g2 = K.resnorm_backward(st.x, f2.h, st.dh, st.dy, f2.stats, st.rows, **st.args())
+    s.synchronize()
+    assert torch.equal(f.h, f2.h) and all(torch.equal(a, b) for a, b in zip(g, g2))
+
+    # captured: replays on new inputs equal the eager call, eager work between them
+    x, res, dh, dy = (t.clone() for t in (st.x, st.res, st.dh, st.dy))
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        f3 = K.resnorm_forward(x, res, st.rows, checkpoint="int8", **st.args())
+        g3 = K.resnorm_backward(f3.x8, f3.h8, dh, dy, f3.stats, st.rows, **st.args())
+    for i in range(4):
+        for t in (x, res, dh, dy):
+            t.copy_(torch.randn(t.shape, generator=torch.Generator().manual_seed(i)).to(t.dtype))
+        fe = K.resnorm_forward(x, res, st.rows, checkpoint="int8", **st.args())
+        ge = K.resnorm_backward(fe.x8, fe.h8, dh, dy, fe.stats, st.rows, **st.args())
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(fe.h, f3.h) and torch.equal(fe.y, f3.y)
+        assert all(torch.equal(a, b) for a, b in zip(ge, g3))
