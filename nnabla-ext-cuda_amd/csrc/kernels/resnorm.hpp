@@ -50,11 +50,17 @@ struct StepPlan {
   int dtype = 0;
   bool layer = false, post = false, pre = false;
   bool kept8 = false;            // backward: x and h are 8-bit copies
-  int tpr = 0, nv = 0;           // threads per row, vectors per thread; 0: the kernels for long rows
+  bool any = false;              // the form of the row kernels for every call (resnorm_rows.cuh)
+  int tpr = 0;                   // threads per row; 0: the kernels for long rows
 };
 
-// Rows a block works on at a time.
-inline int step_rows_per_block(int tpr) { return tpr < 256 ? 256 / tpr : 1; }
+// Threads per row of the kernels that keep a row in registers, a 16-byte vector
+// each.
+#define NBLAHIP_STEP_LAYOUTS(CASE) \
+  CASE(16) CASE(32) CASE(64) CASE(128) CASE(256) CASE(512) CASE(1024)
+
+// Rows a block works on at a time, and its threads.
+inline int step_rows_per_block(int tpr) { return tpr > 0 && tpr < 256 ? 256 / tpr : 1; }
 inline int step_block(int tpr) { return tpr < 256 ? 256 : tpr; }
 
 int launch_step_fwd_f32(const StepPlan &pl, const StepArgs &a, hipStream_t st);
@@ -63,5 +69,8 @@ int launch_step_fwd_bf16(const StepPlan &pl, const StepArgs &a, hipStream_t st);
 int launch_step_bwd_f32(const StepPlan &pl, const StepArgs &a, hipStream_t st);
 int launch_step_bwd_f16(const StepPlan &pl, const StepArgs &a, hipStream_t st);
 int launch_step_bwd_bf16(const StepPlan &pl, const StepArgs &a, hipStream_t st);
+int launch_step_bwd8_f32(const StepPlan &pl, const StepArgs &a, hipStream_t st);
+int launch_step_bwd8_f16(const StepPlan &pl, const StepArgs &a, hipStream_t st);
+int launch_step_bwd8_bf16(const StepPlan &pl, const StepArgs &a, hipStream_t st);
 
 } // namespace nblahip

@@ -1,14 +1,40 @@
-// Launches of the residual step's backward for one storage type.
+// Launches of the residual step's backward for one storage type, from the
+// tensors (Q8 false) or from their 8-bit copies.
 #pragma once
 
 #include <algorithm>
 
-#include "resnorm_long.cuh"
+#include "resnorm_rows.cuh"
 
 namespace nblahip {
 
+template <typename T, bool LN, bool POST, bool PRE, bool Q8, bool ANY>
+bool launch_bwd_rows(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
+  // the one form that does not fit the registers of a block of 1024
+  // (step_bwd_is_long keeps it away)
+  constexpr int MOST = LN && POST && PRE && Q8 && ANY && sizeof(T) == 2 ? 512 : 1024;
+  switch (pl.tpr) {
+#define NBLAHIP_CASE(TPR)                                                                         \
+  case TPR:                                                                                       \
+    if constexpr (TPR <= MOST) {                                                                  \
+      NBLAHIP_LAUNCH("step_bwd_rows_kernel",                                                      \
+                     (step_bwd_rows_kernel<T, LN, POST, PRE, Q8, ANY, TPR>),                      \
+                     dim3(static_cast<unsigned>(a.grid)), dim3(row_block<TPR>()), 0, st, a);      \
+      return true;                                                                                \
+    } else {                                                                                      \
+      return false;                                                                               \
+    }
+    NBLAHIP_STEP_LAYOUTS(NBLAHIP_CASE)
+#undef NBLAHIP_CASE
+  }
+  return false;
+}
+
 template <typename T, bool LN, bool POST, bool PRE, bool Q8>
 int launch_bwd_kind(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
+  if (pl.any ? launch_bwd_rows<T, LN, POST, PRE, Q8, true>(pl, a, st)
+             : launch_bwd_rows<T, LN, POST, PRE, Q8, false>(pl, a, st))
+    return last_launch_status();
   const dim3 rows(static_cast<unsigned>(std::min<int64_t>(a.rows, 1 << 20)));
   NBLAHIP_LAUNCH("step_bwd_long_sums_kernel", (step_bwd_long_sums_kernel<T, LN, POST, PRE, Q8>), rows,
                  dim3(kLongThreads), 0, st, a);
@@ -28,10 +54,8 @@ int launch_bwd_norms(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
   return launch_bwd_kind<T, LN, false, true, Q8>(pl, a, st);
 }
 
-template <typename T> int launch_bwd(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
-  if (pl.layer)
-    return pl.kept8 ? launch_bwd_norms<T, true, true>(pl, a, st) : launch_bwd_norms<T, true, false>(pl, a, st);
-  return pl.kept8 ? launch_bwd_norms<T, false, true>(pl, a, st) : launch_bwd_norms<T, false, false>(pl, a, st);
+template <typename T, bool Q8> int launch_bwd(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
+  return pl.layer ? launch_bwd_norms<T, true, Q8>(pl, a, st) : launch_bwd_norms<T, false, Q8>(pl, a, st);
 }
 
 } // namespace nblahip

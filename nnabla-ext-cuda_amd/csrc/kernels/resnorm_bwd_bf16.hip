@@ -2,6 +2,6 @@
 
 namespace nblahip {
 int launch_step_bwd_bf16(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
-  return launch_bwd<bf16>(pl, a, st);
+  return launch_bwd<bf16, false>(pl, a, st);
 }
 } // namespace nblahip

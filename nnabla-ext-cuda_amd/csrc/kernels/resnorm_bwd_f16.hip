@@ -2,6 +2,6 @@
 
 namespace nblahip {
 int launch_step_bwd_f16(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
-  return launch_bwd<__half>(pl, a, st);
+  return launch_bwd<__half, false>(pl, a, st);
 }
 } // namespace nblahip

@@ -2,6 +2,6 @@
 
 namespace nblahip {
 int launch_step_bwd_f32(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
-  return launch_bwd<float>(pl, a, st);
+  return launch_bwd<float, false>(pl, a, st);
 }
 } // namespace nblahip

@@ -3,12 +3,34 @@
 
 #include <algorithm>
 
-#include "resnorm_long.cuh"
+#include "resnorm_rows.cuh"
 
 namespace nblahip {
 
+template <typename T, bool LN, bool POST, bool PRE, bool COPY, bool ANY>
+bool launch_fwd_rows(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
+  switch (pl.tpr) {
+#define NBLAHIP_CASE(TPR)                                                                         \
+  case TPR:                                                                                       \
+    NBLAHIP_LAUNCH("step_fwd_rows_kernel",                                                        \
+                   (step_fwd_rows_kernel<T, LN, POST, PRE, COPY, ANY, TPR>),                      \
+                   dim3(static_cast<unsigned>(a.grid)), dim3(row_block<TPR>()), 0, st, a);        \
+    return true;
+    NBLAHIP_STEP_LAYOUTS(NBLAHIP_CASE)
+#undef NBLAHIP_CASE
+  }
+  return false;
+}
+
 template <typename T, bool LN, bool POST, bool PRE>
 int launch_fwd_kind(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
+  const bool copy = a.x8 || a.h8;
+  const bool done =
+      pl.any ? copy ? launch_fwd_rows<T, LN, POST, PRE, true, true>(pl, a, st)
+                    : launch_fwd_rows<T, LN, POST, PRE, false, true>(pl, a, st)
+             : copy ? launch_fwd_rows<T, LN, POST, PRE, true, false>(pl, a, st)
+                    : launch_fwd_rows<T, LN, POST, PRE, false, false>(pl, a, st);
+  if (done) return last_launch_status();
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(a.rows, 1 << 20)));
   NBLAHIP_LAUNCH("step_fwd_long_kernel", (step_fwd_long_kernel<T, LN, POST, PRE>), grid,
                  dim3(kLongThreads), 0, st, a);

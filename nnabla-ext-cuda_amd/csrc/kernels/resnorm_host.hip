@@ -2,6 +2,7 @@
 // step and the backward passes from 8-bit copies.  Nothing here allocates,
 // throws or waits for the device.
 #include <algorithm>
+#include <initializer_list>
 
 #include "resnorm.hpp"
 #include "tokens.cuh"
@@ -59,8 +60,30 @@ struct Aliases {
   }
 };
 
+constexpr int kCus = 256;
+
+int vec_of(int dtype) { return dtype == NBLAHIP_F32 ? 4 : 8; }
+
+// As many threads as the row has vectors, up to a block of 1024; longer rows,
+// and those of less than a vector, go to the kernels for long rows.
 void pick_layout(StepPlan &pl, int64_t cols) {
-  pl.tpr = pl.nv = 0;
+  const int64_t vec = vec_of(pl.dtype), vectors = (cols + vec - 1) / vec;
+  pl.tpr = 16;
+  while (pl.tpr < 1024 && pl.tpr < vectors) pl.tpr *= 2;
+  if (pl.tpr < vectors || cols < vec) pl.tpr = 0;
+}
+
+// Whether every address that a 16-byte vector of the tensors (or its 8-bit
+// codes) is at is a multiple of the vector's size.
+bool whole_vectors(int dtype, int64_t cols, std::initializer_list<const void *> tensors,
+                   std::initializer_list<const void *> codes) {
+  const int vec = vec_of(dtype);
+  if (cols % vec != 0) return false;
+  for (const void *p : tensors)
+    if (!aligned16(p)) return false;
+  for (const void *p : codes)
+    if ((reinterpret_cast<uintptr_t>(p) & (vec - 1)) != 0) return false;
+  return true;
 }
 
 // Runs of rows for the backward: rows that share a gate row are cut into
@@ -79,12 +102,24 @@ int64_t shared_gate_rows(const StepArgs &a, int64_t gate_rows) {
   return a.gate_kind == NBLAHIP_GATE_ROWS ? gate_rows : 1;
 }
 
+// The backward's only form whose rows of 1024 threads do not fit the registers.
+bool step_bwd_is_long(const StepPlan &pl, bool any, bool kept8) {
+  return pl.tpr == 1024 && pl.dtype != NBLAHIP_F32 && pl.layer && pl.post && pl.pre && any && kept8;
+}
+
 // The backward's split, and its workspace laid out from `ws` (null: sizes only).
 size_t plan_bwd(StepArgs &a, StepPlan &pl, int64_t gate_rows, char *ws) {
   pick_layout(pl, a.cols);
+  if (step_bwd_is_long(pl, pl.any, pl.kept8)) pl.tpr = 0;
   a.pitch = (a.cols + 7) / 8 * 8;
-  plan_chunks(a, gate_rows, 256, 16);
-  a.grid = static_cast<int>(std::min<int64_t>(a.chunks, 1 << 30));
+  if (pl.tpr == 0) {
+    plan_chunks(a, gate_rows, kCus, 16);
+    a.grid = static_cast<int>(std::min<int64_t>(a.chunks, 1 << 30));
+  } else {
+    const int64_t blocks = kCus * std::max<int64_t>(1, 1024 / step_block(pl.tpr));
+    plan_chunks(a, gate_rows, blocks, step_rows_per_block(pl.tpr));
+    a.grid = static_cast<int>(std::min<int64_t>(a.chunks, blocks));
+  }
   size_t at = 0;
   auto take = [&](int64_t floats) {
     float *p = ws ? reinterpret_cast<float *>(ws + at) : nullptr;
@@ -244,9 +279,9 @@ int run_fwd(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
 }
 int run_bwd(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
   switch (pl.dtype) {
-  case NBLAHIP_F32: return launch_step_bwd_f32(pl, a, st);
-  case NBLAHIP_F16: return launch_step_bwd_f16(pl, a, st);
-  default: return launch_step_bwd_bf16(pl, a, st);
+  case NBLAHIP_F32: return pl.kept8 ? launch_step_bwd8_f32(pl, a, st) : launch_step_bwd_f32(pl, a, st);
+  case NBLAHIP_F16: return pl.kept8 ? launch_step_bwd8_f16(pl, a, st) : launch_step_bwd_f16(pl, a, st);
+  default: return pl.kept8 ? launch_step_bwd8_bf16(pl, a, st) : launch_step_bwd_bf16(pl, a, st);
   }
 }
 
@@ -277,7 +312,12 @@ int step_fwd(StepArgs a, StepPlan pl, int64_t gate_rows, hipStream_t st) {
   al.write(a.h8_scale, qs);
   if (al.bad()) return NBLAHIP_EALIAS;
   pick_layout(pl, a.cols);
-  a.rows_per_gate = a.gate_kind == NBLAHIP_GATE_ROWS ? a.rows / gate_rows : a.rows;
+  pl.any = a.gate_kind == NBLAHIP_GATE_FULL ||
+           !whole_vectors(pl.dtype, a.cols, {a.x, a.res, a.h, a.y}, {a.x8, a.h8});
+  gate_rows = shared_gate_rows(a, gate_rows);
+  const int64_t blocks = kCus * (2048 / step_block(pl.tpr));
+  plan_chunks(a, gate_rows, blocks, step_rows_per_block(pl.tpr));
+  a.grid = static_cast<int>(std::min<int64_t>(a.chunks, blocks));
   return run_fwd(pl, a, st);
 }
 
@@ -294,6 +334,11 @@ int step_bwd(StepArgs a, StepPlan pl, int64_t gate_rows, void *ws, size_t ws_byt
   }
   if (pl.kept8 && !format_ok(a.format8)) return NBLAHIP_EINVAL;
   gate_rows = shared_gate_rows(a, gate_rows);
+  const bool full = a.gate_kind == NBLAHIP_GATE_FULL;
+  pl.any = full || (a.dx && (a.accum & NBLAHIP_ACCUM_DX)) || (a.dres && (a.accum & NBLAHIP_ACCUM_DRES)) ||
+           !whole_vectors(pl.dtype, a.cols, {a.dh, a.dy, a.dx, a.dres}, {}) ||
+           !(pl.kept8 ? whole_vectors(pl.dtype, a.cols, {}, {a.x, a.kept_h})
+                      : whole_vectors(pl.dtype, a.cols, {a.x, a.kept_h}, {}));
   const size_t need = plan_bwd(a, pl, gate_rows, static_cast<char *>(ws));
   if (need && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0 || ws_bytes < need))
     return NBLAHIP_EWORKSPACE;
@@ -302,7 +347,6 @@ int step_bwd(StepArgs a, StepPlan pl, int64_t gate_rows, void *ws, size_t ws_byt
   const size_t kb = pl.kept8 ? n : tb;
   a.groups8 = groups_of(a.cols);
   const size_t qs = static_cast<size_t>(a.rows) * a.groups8;
-  const bool full = a.gate_kind == NBLAHIP_GATE_FULL;
   Aliases al;
   if (reads_x) al.read(a.x, kb, !pl.kept8);
   if (pl.pre) al.read(a.kept_h, kb, !pl.kept8);
@@ -321,6 +365,7 @@ int step_bwd(StepArgs a, StepPlan pl, int64_t gate_rows, void *ws, size_t ws_byt
   for (const float *p : {a.dgamma_post, a.dbeta_post, a.dgamma_pre, a.dbeta_pre}) al.write(p, pb);
   al.write(ws, need);
   if (al.bad()) return NBLAHIP_EALIAS;
+  if (!reads_x) a.x = nullptr;
   if (!pl.pre || !(a.dgamma_pre || a.dbeta_pre)) a.part_pre = nullptr;
   const bool post_sums = (pl.post && (a.dgamma_post || a.dbeta_post)) ||
                          (a.gate_kind == NBLAHIP_GATE_ROWS && a.dgate);
@@ -480,7 +525,11 @@ size_t nblahip_resnorm_bwd_workspace_bytes(int64_t rows, int64_t cols, int gate_
   a.rows = rows;
   a.cols = cols;
   a.gate_kind = gate_kind;
-  return plan_bwd(a, pl, shared_gate_rows(a, gate_rows), nullptr);
+  const int64_t g = shared_gate_rows(a, gate_rows);
+  StepArgs b = a;
+  StepPlan ql = pl;
+  ql.any = ql.kept8 = true; // the call may be of the form that runs as a long row
+  return std::max(plan_bwd(a, pl, g, nullptr), plan_bwd(b, ql, g, nullptr));
 }
 
 int nblahip_resnorm_bwd(const void *x, const uint8_t *x_scale, const void *h, const uint8_t *h_scale,

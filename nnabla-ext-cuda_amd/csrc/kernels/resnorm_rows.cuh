@@ -1,0 +1,664 @@
+// The residual step on rows that fit a block at one 16-byte vector per thread:
+// every tensor crosses HBM once per direction.
+//
+// TPR threads hold a row; blocks of 256 threads take several rows at a time
+// where TPR < 256.  A thread's columns are the same in every row, so the
+// parameters (and, backward, the column sums of the parameter gradients) stay
+// in its registers while the block walks its rows.
+//
+// What bounds it: HBM (6 tensors of 2 bytes an element backward, 4 forward).
+// A row's loads are asked for one row ahead and must stay in flight while the
+// row before is worked on and stored.  This GPU counts loads and stores in one
+// in-order counter per wave, and the compiler can wait for "all but the last
+// n" only where it knows n on every path; after a branch around a load or a
+// store it has to wait for everything, the row's own stores included (and keeps
+// twice the registers: 170 against 80 in the backward).  So the loop has no such
+// branch: every access is a buffer access whose bounds the hardware checks.  An
+// absent tensor, a row past the end and a thread past the columns have no
+// records in range: loads give 0, stores are dropped.
+//
+// ANY = false: rows of whole vectors, 16-byte aligned, no gate per element, no
+// accumulation onto dx / dres: the calls models make.  ANY = true: everything
+// else of these widths.  A row that ends inside a vector is read as the vector
+// that ends where the row ends, shifted down, and written in pieces of 8, 4 and
+// 2 bytes; nothing outside the row is touched.
+#pragma once
+
+#include "resnorm_long.cuh"
+
+namespace nblahip {
+
+// Sums of N values over the TPR threads of a row; every one of them gets the
+// sums.  Rows of several waves go through LDS: two buffers taken in turn, so
+// that one barrier per sum is enough (a wave writes a buffer again only after
+// the barrier of the sum in between, which every wave reaches after its reads).
+template <int TPR, int N> struct RowTotal {
+  static constexpr int kWaves = TPR > kWave ? TPR / kWave : 1;
+  static constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
+  static constexpr int kFloats = TPR > kWave ? 2 * kRows * kWaves * N : 1;
+};
+
+template <int TPR, int N, int CAP>
+__device__ __forceinline__ void row_total(float (&v)[N], float (&lds)[CAP], int &turn) {
+  if constexpr (TPR < kWave) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = group_sum<TPR>(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+    if constexpr (TPR > kWave) {
+      constexpr int W = TPR / kWave;
+      const int wave = threadIdx.x / kWave;
+      float *buf = lds + turn * (CAP / 2);
+      if ((threadIdx.x & (kWave - 1)) == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) buf[wave * N + i] = v[i];
+      }
+      lds_barrier();
+      const float *mine = buf + wave / W * (W * N);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) s += mine[w * N + i];
+        v[i] = s;
+      }
+      turn ^= 1;
+    }
+  }
+}
+
+template <int TPR> constexpr int row_block() { return TPR < 256 ? 256 : TPR; }
+
+typedef __amdgpu_buffer_rsrc_t Buffer;
+constexpr uint32_t kOutside = 0x7fffffffu; // an offset past every buffer here
+constexpr int kStream = 2;                 // non-temporal
+
+// `bytes` bytes at p + off (none where p is null).
+__device__ __forceinline__ Buffer buffer(const void *p, int64_t off, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(static_cast<const char *>(p)) + off, 0,
+                                           p ? static_cast<int>(bytes) : 0, 0x00020000);
+}
+__device__ __forceinline__ Packed buffer_load(Buffer b, uint32_t at) {
+  const native_u4 t = __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0);
+  Packed r;
+  r.v = make_uint4(t.x, t.y, t.z, t.w);
+  return r;
+}
+__device__ __forceinline__ float buffer_load_float(Buffer b, uint32_t at) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(b, at, 0, 0));
+}
+__device__ __forceinline__ void buffer_store(Buffer b, uint32_t at, const Packed &r) {
+  const native_u4 t = {r.v.x, r.v.y, r.v.z, r.v.w};
+  __builtin_amdgcn_raw_buffer_store_b128(t, b, at, 0, kStream);
+}
+__device__ __forceinline__ void buffer_store_float(Buffer b, uint32_t at, float v) {
+  __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), b, at, 0, 0);
+}
+
+__device__ __forceinline__ uint4 shift_down_bits(uint4 v, uint32_t bits) {
+  uint64_t lo = (static_cast<uint64_t>(v.y) << 32) | v.x;
+  uint64_t hi = (static_cast<uint64_t>(v.w) << 32) | v.z;
+  const bool far = bits >= 64;
+  const uint32_t b = bits & 63u;
+  lo = far ? hi : lo;
+  hi = far ? 0 : hi;
+  lo = (lo >> b) | ((hi << 1) << (63u - b));
+  hi >>= b;
+  return make_uint4(static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32),
+                    static_cast<uint32_t>(hi), static_cast<uint32_t>(hi >> 32));
+}
+
+// Makes the compiler finish computing v here: it would otherwise carry both
+// factors of a column sum's update to the end of the row.
+template <int N> __device__ __forceinline__ void settle(float (&v)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) asm volatile("" : "+v"(v[j]));
+}
+
+// Where a thread's vector lies in the rows a block has in hand, in bytes from
+// the first of them: of a tensor of the storage type, of 8-bit codes, of their
+// scales, of a row statistic.  With ANY the thread a row ends in reads the
+// vector `drop` elements further ahead, and writes the first `n` of its own.
+template <typename T, int TPR, bool ANY> struct Place {
+  static constexpr int V = Tok<T>::VEC;
+  static constexpr int RPB = row_block<TPR>() / TPR;
+  static constexpr uint32_t SZ = sizeof(T);
+  uint32_t wide, codes, scale, stat;
+  uint32_t drop; // ANY only
+  int c, n;      // the thread's first column, and how many it has
+  __device__ __forceinline__ Place(const StepArgs &a) {
+    const uint32_t cols = static_cast<uint32_t>(a.cols);
+    const uint32_t sub = TPR >= 256 ? 0 : threadIdx.x / TPR;
+    c = (threadIdx.x % TPR) * V;
+    n = columns_left(a.cols - c, V);
+    drop = ANY && n > 0 ? V - n : 0;
+    wide = n > 0 ? (sub * cols + c - drop) * SZ : kOutside;
+    codes = n > 0 ? sub * cols + c - drop : kOutside;
+    scale = n > 0 ? sub * static_cast<uint32_t>(a.groups8) + c / kAct8Group : kOutside;
+    stat = sub * 4;
+  }
+  __device__ __forceinline__ Packed load(Buffer b) const {
+    Packed r = buffer_load(b, wide);
+    if constexpr (ANY) r.v = shift_down_bits(r.v, drop * 8u * SZ);
+    return r;
+  }
+  // Offsets of the pieces a vector that is cut short is written in.
+  __device__ __forceinline__ uint32_t own(uint32_t at, uint32_t size) const {
+    return n > 0 ? at + drop * size : kOutside;
+  }
+  __device__ __forceinline__ void store(Buffer b, const Packed &r) const {
+    if constexpr (!ANY) {
+      buffer_store(b, wide, r);
+    } else {
+      buffer_store(b, n == V ? wide : kOutside, r);
+      const uint32_t left = static_cast<uint32_t>(n < V ? n : 0); // elements still to write
+      const uint32_t at = own(wide, SZ);
+      const uint32_t four = left & (8 / SZ), two = left & (4 / SZ);
+      const native_u2 t = {r.v.x, r.v.y};
+      __builtin_amdgcn_raw_buffer_store_b64(t, b, four ? at : kOutside, 0, 0);
+      const uint4 q = shift_down_bits(r.v, four ? 64u : 0u);
+      __builtin_amdgcn_raw_buffer_store_b32(q.x, b, two ? at + four * SZ : kOutside, 0, 0);
+      if constexpr (SZ == 2) {
+        const uint32_t w = two ? q.y : q.x;
+        __builtin_amdgcn_raw_buffer_store_b16(static_cast<uint16_t>(w), b,
+                                              left & 1u ? at + (four + two) * SZ : kOutside, 0, 0);
+      }
+    }
+  }
+  // onto what `old` (a buffer without records: nothing) holds there
+  __device__ __forceinline__ void put(Buffer b, Buffer old, const float (&o)[V]) const {
+    if constexpr (ANY) {
+      float sum[V];
+      Tok<T>::unpack(load(old), sum);
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum[j] += o[j];
+      store(b, Tok<T>::pack(sum));
+    } else {
+      store(b, Tok<T>::pack(o));
+    }
+  }
+  __device__ __forceinline__ uint2 load_codes(Buffer b) const {
+    uint2 q = make_uint2(0u, 0u);
+    if constexpr (V == 8) {
+      const native_u2 t = __builtin_amdgcn_raw_buffer_load_b64(b, codes, 0, 0);
+      q = make_uint2(t.x, t.y);
+    } else {
+      q.x = __builtin_amdgcn_raw_buffer_load_b32(b, codes, 0, 0);
+    }
+    if constexpr (ANY) {
+      const uint64_t v = ((static_cast<uint64_t>(q.y) << 32) | q.x) >> (8u * drop);
+      q = make_uint2(static_cast<uint32_t>(v), static_cast<uint32_t>(v >> 32));
+    }
+    return q;
+  }
+  __device__ __forceinline__ void store_codes(Buffer b, uint2 q) const {
+    const uint32_t all = !ANY || n == V ? codes : kOutside;
+    if constexpr (V == 8) {
+      const native_u2 t = {q.x, q.y};
+      __builtin_amdgcn_raw_buffer_store_b64(t, b, all, 0, 0);
+    } else {
+      __builtin_amdgcn_raw_buffer_store_b32(q.x, b, all, 0, 0);
+    }
+    if constexpr (ANY) {
+      const uint32_t left = static_cast<uint32_t>(n < V ? n : 0), at = own(codes, 1);
+      const uint32_t four = left & 4u, two = left & 2u;
+      if constexpr (V == 8) __builtin_amdgcn_raw_buffer_store_b32(q.x, b, four ? at : kOutside, 0, 0);
+      const uint32_t w = four ? q.y : q.x;
+      __builtin_amdgcn_raw_buffer_store_b16(static_cast<uint16_t>(w), b, two ? at + four : kOutside, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b8(static_cast<uint8_t>(two ? w >> 16 : w), b,
+                                           left & 1u ? at + four + two : kOutside, 0, 0);
+    }
+  }
+};
+
+// The factor between the normalized x and its part of h, branch_scale * gate *
+// gamma_post (without a norm: branch_scale * gate), at a thread's columns, and
+// the same of beta_post.  A gate per element comes in later.
+template <int V, bool POST>
+__device__ __forceinline__ void load_branch(const StepArgs &a, int64_t gate_row, int64_t c, int n,
+                                            float (&k)[V]) {
+  float g[V];
+  load_param<V>(POST ? a.gamma_post : nullptr, c, n, k);
+  load_param<V>(a.gate_kind == 1 ? static_cast<const float *>(a.gate) + gate_row * a.cols : nullptr, c,
+                n, g);
+#pragma unroll
+  for (int j = 0; j < V; ++j) k[j] *= a.branch_scale * g[j];
+}
+template <int V>
+__device__ __forceinline__ void load_branch_bias(const StepArgs &a, int64_t gate_row, int64_t c, int n,
+                                                 float (&k)[V]) {
+  float g[V];
+  load_bias<V>(a.beta_post, c, n, k);
+  load_param<V>(a.gate_kind == 1 ? static_cast<const float *>(a.gate) + gate_row * a.cols : nullptr, c,
+                n, g);
+#pragma unroll
+  for (int j = 0; j < V; ++j) k[j] *= a.branch_scale * g[j];
+}
+
+// Rows of [base, base + RPB) that lie before `last`.
+template <int RPB> __device__ __forceinline__ uint32_t rows_in(int64_t base, int64_t last) {
+  const int64_t n = last - base;
+  return n >= RPB ? RPB : n > 0 ? static_cast<uint32_t>(n) : 0u;
+}
+
+// Forward.  A block takes runs of rows (chunks) that share a gate row.
+template <typename T, bool LN, bool POST, bool PRE, bool COPY, bool ANY, int TPR>
+__global__ __launch_bounds__(row_block<TPR>()) void step_fwd_rows_kernel(const StepArgs a) {
+  constexpr int V = Tok<T>::VEC;
+  constexpr int RPB = row_block<TPR>() / TPR;
+  __shared__ float lds[RowTotal<TPR, 1>::kFloats < 2 ? 2 : RowTotal<TPR, 1>::kFloats];
+  int turn = 0;
+  const Place<T, TPR, ANY> pl(a);
+  const uint32_t row_bytes = static_cast<uint32_t>(a.cols) * static_cast<uint32_t>(sizeof(T));
+  const float inv = 1.f / static_cast<float>(a.cols);
+  const uint32_t stat_out = threadIdx.x % TPR == 0 ? pl.stat : kOutside;
+  const uint32_t scale_out = pl.c % kAct8Group == 0 ? pl.scale : kOutside;
+  float gn[V], bn[V], kp[V], kb[V];
+  if constexpr (PRE) load_param<V>(a.gamma_pre, pl.c, pl.n, gn);
+  if constexpr (PRE && LN) load_bias<V>(a.beta_pre, pl.c, pl.n, bn);
+  for (int64_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
+    const int64_t group = chunk / a.chunks_per_gate;
+    const int64_t first = group * a.rows_per_gate + chunk % a.chunks_per_gate * a.chunk_rows;
+    const int64_t last = least(first + a.chunk_rows, (group + 1) * a.rows_per_gate);
+    load_branch<V, POST>(a, group, pl.c, pl.n, kp);
+    if constexpr (POST && LN) load_branch_bias<V>(a, group, pl.c, pl.n, kb);
+    Packed x, r, gf;
+    auto ask = [&](int64_t base) {
+      const int64_t off = base * a.cols * static_cast<int64_t>(sizeof(T));
+      const uint32_t bytes = rows_in<RPB>(base, last) * row_bytes;
+      x = pl.load(buffer(a.x, off, bytes));
+      r = pl.load(buffer(a.res, off, bytes));
+      if constexpr (ANY) gf = pl.load(buffer(a.gate_kind == 2 ? a.gate : nullptr, off, bytes));
+    };
+    ask(first);
+#pragma unroll 1
+    for (int64_t base = first; base < last; base += RPB) {
+      const uint32_t rows = rows_in<RPB>(base, last), bytes = rows * row_bytes;
+      const int64_t off = base * a.cols * static_cast<int64_t>(sizeof(T));
+      float h[V], q[V];
+      float m1 = 0.f, v1 = 0.f, m2 = 0.f, v2 = 0.f;
+      Tok<T>::unpack(x, h);
+      Tok<T>::unpack(r, q);
+#pragma unroll
+      for (int j = 0; j < V; ++j) q[j] *= a.res_scale;
+      auto copy = [&](const float (&v)[V], void *codes, void *scales) {
+        uint32_t code;
+        const uint2 w = act8_encode<V>(v, a.format8, code);
+        const Buffer to = buffer(codes, base * a.cols, rows * static_cast<uint32_t>(a.cols));
+        pl.store_codes(to, w);
+        __builtin_amdgcn_raw_buffer_store_b8(
+            static_cast<uint8_t>(code),
+            buffer(scales, base * a.groups8, rows * static_cast<uint32_t>(a.groups8)), scale_out, 0, 0);
+      };
+      if constexpr (COPY) copy(h, a.x8, a.x8_scale);
+      float g[V];
+      if constexpr (ANY) {
+        Tok<T>::unpack(gf, g);
+#pragma unroll
+        for (int j = 0; j < V; ++j) g[j] = a.gate_kind == 2 ? g[j] : 1.f;
+        settle(g);
+      }
+      settle(h);
+      settle(q);
+      ask(base + RPB);
+      auto moments = [&](float &mean, float &var) {
+        float s[1] = {0.f};
+        if constexpr (LN) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) s[0] += h[j];
+          row_total<TPR, 1>(s, lds, turn);
+          mean = s[0] * inv;
+        }
+        s[0] = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          float d = LN ? h[j] - mean : h[j];
+          if constexpr (LN && ANY) d = j < pl.n ? d : 0.f;
+          s[0] = fmaf(d, d, s[0]);
+        }
+        if constexpr (LN && !ANY) s[0] = pl.n > 0 ? s[0] : 0.f;
+        row_total<TPR, 1>(s, lds, turn);
+        var = s[0] * inv;
+      };
+      float rho = 1.f;
+      if constexpr (POST) {
+        moments(m1, v1);
+        rho = inv_std(v1, a.eps);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float u = (POST && LN ? h[j] - m1 : h[j]) * rho;
+        if constexpr (ANY) {
+          h[j] = fmaf(POST && LN ? fmaf(u, kp[j], kb[j]) : u * kp[j], g[j], q[j]);
+        } else {
+          if constexpr (POST && LN) q[j] += kb[j];
+          h[j] = fmaf(u, kp[j], q[j]);
+        }
+      }
+      const Packed hp = Tok<T>::pack(h);
+      pl.store(buffer(a.h, off, bytes), hp);
+      if constexpr (COPY && PRE) {
+        float hv[V];
+        Tok<T>::unpack(hp, hv);
+        copy(hv, a.h8, a.h8_scale);
+      }
+      if constexpr (PRE) {
+        moments(m2, v2);
+        const float rho2 = inv_std(v2, a.eps);
+        float y[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          y[j] = LN ? fmaf((h[j] - m2) * rho2, gn[j], bn[j]) : h[j] * rho2 * gn[j];
+        pl.store(buffer(a.y, off, bytes), Tok<T>::pack(y));
+      }
+      if constexpr (POST) {
+        if constexpr (LN) buffer_store_float(buffer(a.mean_post, 4 * base, 4 * rows), stat_out, m1);
+        buffer_store_float(buffer(a.var_post, 4 * base, 4 * rows), stat_out, v1);
+      }
+      if constexpr (PRE) {
+        if constexpr (LN) buffer_store_float(buffer(a.mean_pre, 4 * base, 4 * rows), stat_out, m2);
+        buffer_store_float(buffer(a.var_pre, 4 * base, 4 * rows), stat_out, v2);
+      }
+    }
+  }
+}
+
+// A kept tensor's vector as it was loaded: storage type, or an 8-bit copy.
+template <typename T, bool Q8, int TPR, bool ANY> struct Kept {
+  Packed p;
+  __device__ __forceinline__ void ask(const StepArgs &a, const void *data, const uint8_t *, int64_t base,
+                                      uint32_t rows, const Place<T, TPR, ANY> &pl) {
+    p = pl.load(buffer(data, base * a.cols * static_cast<int64_t>(sizeof(T)),
+                       rows * static_cast<uint32_t>(a.cols) * static_cast<uint32_t>(sizeof(T))));
+  }
+  __device__ __forceinline__ void get(const StepArgs &, float (&o)[Tok<T>::VEC]) const {
+    Tok<T>::unpack(p, o);
+  }
+  // Hides the value from the optimiser, so that its widened form is made anew
+  // where it is needed instead of being kept in twice the registers.
+  __device__ __forceinline__ void pin() {
+    if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(p.v.x), "+v"(p.v.y), "+v"(p.v.z), "+v"(p.v.w));
+  }
+};
+template <typename T, int TPR, bool ANY> struct Kept<T, true, TPR, ANY> {
+  uint2 q;
+  uint32_t code;
+  __device__ __forceinline__ void ask(const StepArgs &a, const void *data, const uint8_t *scales,
+                                      int64_t base, uint32_t rows, const Place<T, TPR, ANY> &pl) {
+    q = pl.load_codes(buffer(data, base * a.cols, rows * static_cast<uint32_t>(a.cols)));
+    code = __builtin_amdgcn_raw_buffer_load_b8(
+        buffer(scales, base * a.groups8, rows * static_cast<uint32_t>(a.groups8)), pl.scale, 0, 0);
+  }
+  __device__ __forceinline__ void get(const StepArgs &a, float (&o)[Tok<T>::VEC]) const {
+    act8_decode<Tok<T>::VEC>(q, code, a.format8, o);
+  }
+  __device__ __forceinline__ void pin() { asm volatile("" : "+v"(q.x), "+v"(q.y), "+v"(code)); }
+};
+
+// Column sums of one kind for the thread's columns: in registers, or in LDS where
+// a block of 1024 threads has none left for them (16 bytes of LDS traffic per
+// column and row against 24 of HBM's for the whole CU: it does not show).
+template <int V, int TPR, bool IN_LDS> struct ColumnSum {
+  float v[V];
+  __device__ __forceinline__ void clear(float4 *) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = 0.f;
+  }
+  __device__ __forceinline__ void add(float4 *, int j, float a, float b) { v[j] = fmaf(a, b, v[j]); }
+  __device__ __forceinline__ void load(float4 *) {}
+  __device__ __forceinline__ void save(float4 *) { settle(v); }
+  __device__ __forceinline__ void get(const float4 *, float (&o)[V]) const {
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = v[j];
+  }
+};
+template <int V, int TPR> struct ColumnSum<V, TPR, true> {
+  float v[V]; // only between load and save
+  __device__ __forceinline__ void clear(float4 *lds) {
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) lds[j * TPR + threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  __device__ __forceinline__ void load(float4 *lds) {
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) {
+      const float4 t = lds[j * TPR + threadIdx.x];
+      v[4 * j] = t.x; v[4 * j + 1] = t.y; v[4 * j + 2] = t.z; v[4 * j + 3] = t.w;
+    }
+  }
+  __device__ __forceinline__ void add(float4 *, int j, float a, float b) { v[j] = fmaf(a, b, v[j]); }
+  __device__ __forceinline__ void save(float4 *lds) {
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j)
+      lds[j * TPR + threadIdx.x] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  }
+  __device__ __forceinline__ void get(const float4 *lds, float (&o)[V]) const {
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) {
+      const float4 t = lds[j * TPR + threadIdx.x];
+      o[4 * j] = t.x; o[4 * j + 1] = t.y; o[4 * j + 2] = t.z; o[4 * j + 3] = t.w;
+    }
+  }
+};
+
+// Backward.  Each input vector is asked for again, for the next row, right
+// after its last use.
+template <typename T, bool LN, bool POST, bool PRE, bool Q8, bool ANY, int TPR>
+__global__ __launch_bounds__(row_block<TPR>()) void step_bwd_rows_kernel(const StepArgs a) {
+  constexpr int V = Tok<T>::VEC;
+  constexpr int RPB = row_block<TPR>() / TPR;
+  constexpr int S = LN ? 2 : 1; // row sums per norm, column sums per norm
+  __shared__ float lds[RowTotal<TPR, S>::kFloats < 2 ? 2 : RowTotal<TPR, S>::kFloats];
+  __shared__ float fold[RPB > 1 ? 256 * V : 1];
+  int turn = 0;
+  const Place<T, TPR, ANY> pl(a);
+  const uint32_t row_bytes = static_cast<uint32_t>(a.cols) * static_cast<uint32_t>(sizeof(T));
+  const float inv = 1.f / static_cast<float>(a.cols);
+  float kp[V], gn[V];
+  // C, A: sums of gradient times normalized value; E, B: of the gradient (LN)
+  constexpr bool TIGHT = TPR == 1024 && V == 8;
+  constexpr bool EB_LDS = LN && TIGHT, A_LDS = TIGHT && (ANY || (LN && Q8));
+  constexpr bool C_LDS = TIGHT && LN && (ANY || Q8);
+  constexpr bool RELOAD = TIGHT && ANY && LN && POST; // gamma_pre: read per row
+  __shared__ float4 eb_lds[EB_LDS ? 2 * TPR * V / 4 : 1], a_lds[A_LDS ? TPR * V / 4 : 1],
+      c_lds[C_LDS ? TPR * V / 4 : 1];
+  float4 *const e_lds = eb_lds, *const b_lds = eb_lds + (EB_LDS ? TPR * V / 4 : 0);
+  ColumnSum<V, TPR, C_LDS> C;
+  ColumnSum<V, TPR, EB_LDS> E, B;
+  ColumnSum<V, TPR, A_LDS> A;
+  if constexpr (PRE && !RELOAD) load_param<V>(a.gamma_pre, pl.c, pl.n, gn);
+  C.clear(c_lds);
+  E.clear(e_lds);
+
+  Kept<T, Q8, TPR, ANY> x, h;
+  Packed dh, dy, gf;
+  float m1 = 0.f, v1 = 0.f, m2 = 0.f, v2 = 0.f;
+  // Column sums (times `scale`) of the block's rows-at-a-time to `out`; every
+  // thread of the block is here.
+  auto flush = [&](float *out, const float (&s)[V], float scale) {
+    if constexpr (RPB == 1) {
+      if (pl.c < a.pitch) {
+#pragma unroll
+        for (int j = 0; j < V; j += 4)
+          *reinterpret_cast<float4 *>(out + pl.c + j) =
+              make_float4(s[j] * scale, s[j + 1] * scale, s[j + 2] * scale, s[j + 3] * scale);
+      }
+    } else {
+      lds_barrier();
+#pragma unroll
+      for (int j = 0; j < V; ++j) fold[j * 256 + threadIdx.x] = s[j];
+      lds_barrier();
+      // 256 threads over the TPR * V columns of the tile, RPB values each
+      for (int i = threadIdx.x; i < TPR * V; i += 256) {
+        const int j = i / TPR, l = i % TPR;
+        float t = 0.f;
+#pragma unroll
+        for (int q = 0; q < RPB; ++q) t += fold[j * 256 + q * TPR + l];
+        if (l * V + j < a.pitch) out[l * V + j] = t * scale;
+      }
+    }
+  };
+
+  for (int64_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
+    const int64_t group = chunk / a.chunks_per_gate;
+    const int64_t first = group * a.rows_per_gate + chunk % a.chunks_per_gate * a.chunk_rows;
+    const int64_t last = least(first + a.chunk_rows, (group + 1) * a.rows_per_gate);
+    A.clear(a_lds);
+    B.clear(b_lds);
+    load_branch<V, POST>(a, group, pl.c, pl.n, kp);
+    auto ask_pre = [&](int64_t base) {
+      const uint32_t rows = rows_in<RPB>(base, last);
+      const int64_t off = base * a.cols * static_cast<int64_t>(sizeof(T));
+      if constexpr (PRE) {
+        h.ask(a, a.kept_h, a.kept_h_scale, base, rows, pl);
+        dy = pl.load(buffer(a.dy, off, rows * row_bytes));
+        if constexpr (LN) m2 = buffer_load_float(buffer(a.mean_pre, 4 * base, 4 * rows), pl.stat);
+        v2 = buffer_load_float(buffer(a.var_pre, 4 * base, 4 * rows), pl.stat);
+      }
+      dh = pl.load(buffer(a.dh, off, rows * row_bytes));
+    };
+    auto ask_post = [&](int64_t base) {
+      const uint32_t rows = rows_in<RPB>(base, last);
+      x.ask(a, a.x, a.kept_x_scale, base, rows, pl);
+      if constexpr (ANY)
+        gf = pl.load(buffer(a.gate_kind == 2 ? a.gate : nullptr,
+                            base * a.cols * static_cast<int64_t>(sizeof(T)), rows * row_bytes));
+      if constexpr (POST) {
+        if constexpr (LN) m1 = buffer_load_float(buffer(a.mean_post, 4 * base, 4 * rows), pl.stat);
+        v1 = buffer_load_float(buffer(a.var_post, 4 * base, 4 * rows), pl.stat);
+      }
+    };
+    ask_pre(first);
+    ask_post(first);
+#pragma unroll 1
+    for (int64_t base = first; base < last; base += RPB) {
+      const uint32_t rows = rows_in<RPB>(base, last);
+      const int64_t off = base * a.cols * static_cast<int64_t>(sizeof(T));
+      const bool in = RPB == 1 || pl.stat < 4 * rows;
+      float t[V];
+      if constexpr (PRE) {
+        const float rho = in ? inv_std(v2, a.eps) : 0.f, mu = m2;
+        float s[S], hh[V], d[V];
+#pragma unroll
+        for (int i = 0; i < S; ++i) s[i] = 0.f;
+        h.get(a, hh);
+        Tok<T>::unpack(dy, d);
+        if constexpr (RELOAD) load_param<V>(a.gamma_pre, pl.c, pl.n, gn);
+        C.load(c_lds);
+        if constexpr (LN) E.load(e_lds);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          hh[j] = (LN ? hh[j] - mu : hh[j]) * rho;
+          C.add(c_lds, j, d[j], hh[j]);
+          if constexpr (LN) E.add(e_lds, j, d[j], 1.f);
+          d[j] *= gn[j];
+          if constexpr (LN) s[S - 1] += d[j];
+          s[0] = fmaf(d[j], hh[j], s[0]);
+        }
+        C.save(c_lds);
+        if constexpr (LN) E.save(e_lds);
+        h.pin();
+        if constexpr (sizeof(T) == 2)
+          asm volatile("" : "+v"(dy.v.x), "+v"(dy.v.y), "+v"(dy.v.z), "+v"(dy.v.w));
+        row_total<TPR, S>(s, lds, turn);
+        const float s2 = s[0] * inv, s1 = LN ? s[S - 1] * inv : 0.f;
+        if constexpr (RELOAD) load_param<V>(a.gamma_pre, pl.c, opaque(pl.n), gn);
+        h.get(a, hh);
+        Tok<T>::unpack(dy, d);
+        Tok<T>::unpack(dh, t);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          hh[j] = (LN ? hh[j] - mu : hh[j]) * rho;
+          t[j] = fmaf(rho, fmaf(d[j], gn[j], -(LN ? fmaf(hh[j], s2, s1) : hh[j] * s2)), t[j]);
+        }
+      } else {
+        Tok<T>::unpack(dh, t);
+      }
+      settle(t);
+      ask_pre(base + RPB);
+      {
+        float o[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = a.res_scale * t[j];
+        pl.put(buffer(a.dres, off, rows * row_bytes),
+               buffer(a.accum & NBLAHIP_ACCUM_DRES ? a.dres : nullptr, off, rows * row_bytes), o);
+      }
+      const float rho = POST ? in ? inv_std(v1, a.eps) : 0.f : 1.f, mu = POST ? m1 : 0.f;
+      float m[S], xh[V];
+#pragma unroll
+      for (int i = 0; i < S; ++i) m[i] = 0.f;
+      x.get(a, xh);
+      if constexpr (POST) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) xh[j] = (LN ? xh[j] - mu : xh[j]) * rho;
+      }
+      if constexpr (ANY) {
+        const bool full = a.gate_kind == 2;
+        float g[V];
+        if constexpr (POST && LN) load_bias<V>(full ? a.beta_post : nullptr, pl.c, pl.n, g);
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          g[j] = t[j] * (POST && LN ? fmaf(xh[j], kp[j], a.branch_scale * g[j]) : xh[j] * kp[j]);
+        pl.put(buffer(full ? a.dgate : nullptr, off, rows * row_bytes),
+               buffer(full && (a.accum & NBLAHIP_ACCUM_DGATE) ? a.dgate : nullptr, off, rows * row_bytes), g);
+        Tok<T>::unpack(gf, g);
+#pragma unroll
+        for (int j = 0; j < V; ++j) t[j] *= full ? g[j] : 1.f;
+      }
+      // branch_scale and a shared gate are multiplied in after the column sums
+      A.load(a_lds);
+      if constexpr (LN && POST) B.load(b_lds);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        A.add(a_lds, j, t[j], xh[j]);
+        if constexpr (LN && POST) B.add(b_lds, j, in ? t[j] : 0.f, 1.f);
+        t[j] *= kp[j];
+        if constexpr (POST) {
+          if constexpr (LN) m[S - 1] += t[j];
+          m[0] = fmaf(t[j], xh[j], m[0]);
+        }
+      }
+      // (Columns beyond the row's end carry finite leftovers here; their gamma is
+      // zero, so no row sum has them, and no sum or element of theirs is stored.)
+      A.save(a_lds);
+      if constexpr (LN && POST) B.save(b_lds);
+      if constexpr (POST) {
+        x.pin();
+        row_total<TPR, S>(m, lds, turn);
+        const float s2 = m[0] * inv, s1 = LN ? m[S - 1] * inv : 0.f;
+        x.get(a, xh);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          xh[j] = (LN ? xh[j] - mu : xh[j]) * rho;
+          t[j] = rho * (t[j] - (LN ? fmaf(xh[j], s2, s1) : xh[j] * s2));
+        }
+      }
+      settle(t);
+      ask_post(base + RPB);
+      pl.put(buffer(a.dx, off, rows * row_bytes),
+             buffer(a.accum & NBLAHIP_ACCUM_DX ? a.dx : nullptr, off, rows * row_bytes), t);
+    }
+    if (a.part_post) {
+      float *out = a.part_post + chunk * S * a.pitch;
+      float s[V];
+      A.get(a_lds, s);
+      flush(out, s, a.branch_scale);
+      if constexpr (LN) {
+        B.get(b_lds, s);
+        flush(out + a.pitch, s, a.branch_scale);
+      }
+    }
+  }
+  if (PRE && a.part_pre) {
+    float *out = a.part_pre + static_cast<int64_t>(blockIdx.x) * S * a.pitch;
+    float s[V];
+    C.get(c_lds, s);
+    flush(out, s, 1.f);
+    if constexpr (LN) {
+      E.get(e_lds, s);
+      flush(out + a.pitch, s, 1.f);
+    }
+  }
+}
+
+} // namespace nblahip

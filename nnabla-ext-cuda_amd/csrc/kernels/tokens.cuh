@@ -29,6 +29,14 @@ __device__ __forceinline__ int columns_left(int64_t remaining, int vec) {
 }
 __device__ __forceinline__ int64_t least(int64_t a, int64_t b) { return a < b ? a : b; }
 
+// The element-by-element paths at a row's end are rare.  Hiding their count keeps
+// the compiler from working out their masks and addresses ahead of the row loop,
+// which costs more registers than the loop itself.
+__device__ __forceinline__ int opaque(int n) {
+  asm volatile("" : "+v"(n));
+  return n;
+}
+
 // VEC elements as they are stored: 16 bytes.
 struct Packed {
   uint4 v;
@@ -106,6 +114,7 @@ template <typename T> struct Tok {
       const any_u4 t = {r.v.x, r.v.y, r.v.z, r.v.w};
       __builtin_nontemporal_store(t, reinterpret_cast<any_u4 *>(p));
     } else if (n > 0) {
+      n = opaque(n);
       const uint32_t w[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
 #pragma unroll
       for (int j = 0; j < VEC - 1; ++j) {
@@ -137,8 +146,12 @@ template <typename T> struct Tok {
 template <int VEC>
 __device__ __forceinline__ void load_param(const float *p, int64_t at, int n, float (&o)[VEC]) {
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) o[j] = (!p && j < n) ? 1.f : 0.f;
-  if (p) {
+  for (int j = 0; j < VEC; ++j) o[j] = 0.f;
+  if (!p) {
+    n = opaque(n);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) o[j] = j < n ? 1.f : 0.f;
+  } else {
     p += at;
     if (n >= VEC) {
 #pragma unroll
@@ -146,7 +159,8 @@ __device__ __forceinline__ void load_param(const float *p, int64_t at, int n, fl
         const any_f4 t = reinterpret_cast<const any_f4 *>(p)[i];
         o[4 * i] = t.x; o[4 * i + 1] = t.y; o[4 * i + 2] = t.z; o[4 * i + 3] = t.w;
       }
-    } else {
+    } else if (n > 0) {
+      n = opaque(n);
 #pragma unroll
       for (int j = 0; j < VEC - 1; ++j)
         if (j < n) o[j] = p[j];
@@ -286,6 +300,7 @@ template <int VEC> __device__ __forceinline__ void act8_store(uint8_t *p, int n,
       *reinterpret_cast<any_u1 *>(p) = q.x;
     }
   } else if (n > 0) {
+    n = opaque(n);
     const uint32_t w[2] = {q.x, q.y};
 #pragma unroll
     for (int j = 0; j < VEC - 1; ++j)

@@ -76,6 +76,18 @@ def test_from_eight_bits(post, pre, gate, norm, dtype, kept):
         run(Step(rows, cols, dtype, norm, post, pre, True, gate), kept)
 
 
+@pytest.mark.parametrize("kept", [None, "int8", "e4m3"])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize("post,pre", [(True, True), (True, False), (False, True)])
+def test_blocks_of_1024_threads(post, pre, norm, dtype, kept):
+    """The widest rows held in registers, where sums move to LDS or the call to
+    the kernels for long rows: whole vectors, ragged, a gate per element."""
+    wide = 1 if dtype == "f32" else 2
+    for cols, gate in ((4096 * wide, "sample"), (2304 * wide + 1, "none"), (3000 * wide, "full")):
+        run(Step(18, cols, dtype, norm, post, pre, True, gate, samples=3), kept)
+
+
 @pytest.mark.parametrize("norm", ["rms", "layer"])
 def test_without_parameters(norm):
     run(Step(40, 520, "f16", norm, gate="sample", samples=4, affine=False))
