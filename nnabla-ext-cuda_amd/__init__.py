@@ -622,12 +622,13 @@ _token_dtypes = {}
 
 
 def _token_dtype(t):
-    if not _token_dtypes:
-        import torch
-        _token_dtypes.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
     code = _token_dtypes.get(t)
     if code is None:
-        raise TypeError(f"unsupported activation dtype {t}")
+        import torch
+        _token_dtypes.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+        code = _token_dtypes.get(t)
+        if code is None:
+            raise TypeError(f"unsupported activation dtype {t}")
     return code
 
 
@@ -640,33 +641,32 @@ def _act8_format(a):
     raise TypeError(f"8-bit codes must be int8 or float8_e4m3fn, not {a.codes.dtype}")
 
 
-class _On:
-    """Current device = the tensors' device, and its current stream, for one
-    call; every tensor must be contiguous and on that device."""
-    __slots__ = ("device", "guard")
-
-    def __init__(self, first, *rest):
-        import torch
-        self.device = d = first.device
-        if d.type != "cuda":
-            raise TypeError(f"tensors must be on a GPU, not on {d}")
-        for t in (first,) + rest:
-            if t is None:
-                continue
-            if t.device != d:
-                raise ValueError(f"tensors on {d} and on {t.device} in one call")
+def _one_gpu(first, *rest):
+    """Index of the GPU that all tensors (None: none) are on, contiguous."""
+    index = first.get_device()
+    if index < 0:
+        raise TypeError(f"tensors must be on a GPU, not on {first.device}")
+    if not first.is_contiguous():
+        raise ValueError("tensors must be contiguous")
+    for t in rest:
+        if t is not None:
+            if t.get_device() != index:
+                raise ValueError(f"tensors on {first.device} and on {t.device} in one call")
             if not t.is_contiguous():
                 raise ValueError("tensors must be contiguous")
-        self.guard = None if d.index == torch.cuda.current_device() else torch.cuda.device(d)
+    return index
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return _stream()
 
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(index, fn, *args):
+    """fn(*args, stream) on GPU `index`, on that GPU's current stream."""
+    import torch
+    if index == torch.cuda.current_device():
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if code != 0:
+        check(code)
 
 
 def _rows_cols(t, outer):
@@ -698,17 +698,21 @@ def _check_kept(k, name, rows, cols, dtype):
     return k, None, 0
 
 
+def _new_act8(x, rows, cols, f):
+    import torch
+    return Act8(torch.empty(x.shape, dtype=torch.int8 if f == 1 else torch.float8_e4m3fn,
+                            device=x.device),
+                torch.empty((rows, (cols + 31) // 32), dtype=torch.uint8, device=x.device))
+
+
 def act8_pack(x, outer, format="int8"):
     """8-bit copy of x: Act8(codes like x, scales [outer, ceil(cols / 32)])."""
-    import torch
     rows, cols = _rows_cols(x, outer)
     f = ACT8_FORMATS[format]
-    with _On(x) as st:
-        codes = torch.empty(x.shape, dtype=torch.int8 if f == 1 else torch.float8_e4m3fn, device=x.device)
-        scales = torch.empty((rows, (cols + 31) // 32), dtype=torch.uint8, device=x.device)
-        check(lib().nblahip_act8_pack(_ptr(x), _ptr(codes), _ptr(scales), rows, cols, f,
-                                      _token_dtype(x.dtype), st))
-    return Act8(codes, scales)
+    dt, gpu = _token_dtype(x.dtype), _one_gpu(x)
+    a = _new_act8(x, rows, cols, f)
+    _call(gpu, lib().nblahip_act8_pack, _ptr(x), _ptr(a.codes), _ptr(a.scales), rows, cols, f, dt)
+    return a
 
 
 def act8_unpack(a, outer, dtype, out=None):
@@ -716,12 +720,11 @@ def act8_unpack(a, outer, dtype, out=None):
     import torch
     rows, cols = _rows_cols(a.codes, outer)
     codes, scales, f = _check_kept(a, "a", rows, cols, dtype)
-    with _On(codes, scales, out) as st:
-        if out is None:
-            out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
-        _like(out, rows * cols, dtype, "out")
-        check(lib().nblahip_act8_unpack(_ptr(codes), _ptr(scales), _ptr(out), rows, cols, f,
-                                        _token_dtype(dtype), st))
+    dt, gpu = _token_dtype(dtype), _one_gpu(codes, scales, out)
+    if out is None:
+        out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    _like(out, rows * cols, dtype, "out")
+    _call(gpu, lib().nblahip_act8_unpack, _ptr(codes), _ptr(scales), _ptr(out), rows, cols, f, dt)
     return out
 
 
@@ -730,11 +733,11 @@ def rms_forward(x, gamma, outer, eps=1e-5, y=None):
     import torch
     rows, cols = _rows_cols(x, outer)
     dt = _token_dtype(x.dtype)
-    with _On(x, gamma, y) as st:
-        _like(gamma, cols, torch.float32, "gamma")
-        y = torch.empty_like(x) if y is None else _like(y, rows * cols, x.dtype, "y")
-        ms = torch.empty(rows, dtype=torch.float32, device=x.device)
-        check(lib().nblahip_rms_fwd(_ptr(x), _ptr(gamma), _ptr(y), _ptr(ms), rows, cols, eps, dt, st))
+    gpu = _one_gpu(x, gamma, y)
+    _like(gamma, cols, torch.float32, "gamma")
+    y = torch.empty_like(x) if y is None else _like(y, rows * cols, x.dtype, "y")
+    ms = torch.empty(rows, dtype=torch.float32, device=x.device)
+    _call(gpu, lib().nblahip_rms_fwd, _ptr(x), _ptr(gamma), _ptr(y), _ptr(ms), rows, cols, eps, dt)
     return y, ms
 
 
@@ -746,19 +749,18 @@ def rms_backward(x, dy, gamma, ms, outer, eps=1e-5, dx=None, dgamma=None, accum=
     rows, cols = _rows_cols(dy, outer)
     dt = _token_dtype(dy.dtype)
     xd, xs, f = _check_kept(x, "x", rows, cols, dy.dtype)
-    with _On(dy, xd, xs, gamma, ms, dx, dgamma, ws) as st:
-        _like(gamma, cols, torch.float32, "gamma")
-        _like(ms, rows, torch.float32, "ms")
-        dx = None if not need[0] else torch.empty_like(dy) if dx is None else _like(
-            dx, rows * cols, dy.dtype, "dx")
-        dgamma = None if not need[1] else torch.empty(
-            cols, dtype=torch.float32, device=dy.device) if dgamma is None else _like(
-                dgamma, cols, torch.float32, "dgamma")
-        if ws is None:
-            ws = _workspace(lib().nblahip_rms_bwd_workspace_bytes(rows, cols, dt), dy.device)
-        check(lib().nblahip_rms_bwd(_ptr(xd), _ptr(xs), f, _ptr(dy), _ptr(gamma), _ptr(ms), _ptr(dx),
-                                    _ptr(dgamma), int(accum[0]), int(accum[1]), rows, cols, eps, dt,
-                                    _ptr(ws), ws.numel(), st))
+    gpu = _one_gpu(dy, xd, xs, gamma, ms, dx, dgamma, ws)
+    _like(gamma, cols, torch.float32, "gamma")
+    _like(ms, rows, torch.float32, "ms")
+    dx = None if not need[0] else torch.empty_like(dy) if dx is None else _like(
+        dx, rows * cols, dy.dtype, "dx")
+    dgamma = None if not need[1] else torch.empty(
+        cols, dtype=torch.float32, device=dy.device) if dgamma is None else _like(
+            dgamma, cols, torch.float32, "dgamma")
+    if ws is None:
+        ws = _workspace(lib().nblahip_rms_bwd_workspace_bytes(rows, cols, dt), dy.device)
+    _call(gpu, lib().nblahip_rms_bwd, _ptr(xd), _ptr(xs), f, _ptr(dy), _ptr(gamma), _ptr(ms), _ptr(dx),
+          _ptr(dgamma), int(accum[0]), int(accum[1]), rows, cols, eps, dt, _ptr(ws), ws.nbytes)
     return dx, dgamma
 
 
@@ -771,21 +773,20 @@ def ln_backward_act8(x8, dy, gamma, mean, var, outer, eps=1e-5, dx=None, dgamma=
     rows, cols = _rows_cols(dy, outer)
     dt = _token_dtype(dy.dtype)
     xd, xs, f = _check_kept(x8, "x8", rows, cols, dy.dtype)
-    with _On(dy, xd, xs, gamma, mean, var, dx, dgamma, dbeta, ws) as st:
-        _like(gamma, cols, torch.float32, "gamma")
-        _like(mean, rows, torch.float32, "mean")
-        _like(var, rows, torch.float32, "var")
-        dx = None if not need[0] else torch.empty_like(dy) if dx is None else _like(
-            dx, rows * cols, dy.dtype, "dx")
-        par = [None if not need[i] else torch.empty(cols, dtype=torch.float32, device=dy.device)
-               if t is None else _like(t, cols, torch.float32, n)
-               for i, t, n in ((1, dgamma, "dgamma"), (2, dbeta, "dbeta"))]
-        if ws is None:
-            ws = _workspace(lib().nblahip_ln_bwd_act8_workspace_bytes(rows, cols, dt), dy.device)
-        check(lib().nblahip_ln_bwd_act8(_ptr(xd), _ptr(xs), f, _ptr(dy), _ptr(gamma), _ptr(mean),
-                                        _ptr(var), _ptr(dx), _ptr(par[0]), _ptr(par[1]),
-                                        int(accum[0]), int(accum[1]), int(accum[2]), rows, cols, eps,
-                                        dt, _ptr(ws), ws.numel(), st))
+    gpu = _one_gpu(dy, xd, xs, gamma, mean, var, dx, dgamma, dbeta, ws)
+    _like(gamma, cols, torch.float32, "gamma")
+    _like(mean, rows, torch.float32, "mean")
+    _like(var, rows, torch.float32, "var")
+    dx = None if not need[0] else torch.empty_like(dy) if dx is None else _like(
+        dx, rows * cols, dy.dtype, "dx")
+    par = [None if not need[i] else torch.empty(cols, dtype=torch.float32, device=dy.device)
+           if t is None else _like(t, cols, torch.float32, n)
+           for i, t, n in ((1, dgamma, "dgamma"), (2, dbeta, "dbeta"))]
+    if ws is None:
+        ws = _workspace(lib().nblahip_ln_bwd_act8_workspace_bytes(rows, cols, dt), dy.device)
+    _call(gpu, lib().nblahip_ln_bwd_act8, _ptr(xd), _ptr(xs), f, _ptr(dy), _ptr(gamma), _ptr(mean),
+          _ptr(var), _ptr(dx), _ptr(par[0]), _ptr(par[1]), int(accum[0]), int(accum[1]), int(accum[2]),
+          rows, cols, eps, dt, _ptr(ws), ws.nbytes)
     return dx, par[0], par[1]
 
 
@@ -807,20 +808,21 @@ def _gate_args(gate, rows, cols, dtype):
     return 1, g
 
 
-def _step_params(cols, post, pre, norm, gamma_post, beta_post, gamma_pre, beta_pre):
+def _step_params(cols, post, pre, kind, gamma_post, beta_post, gamma_pre, beta_pre):
     import torch
     if not (post or pre):
         raise ValueError("a step has the norm after the block (post), the one before the next (pre) "
                          "or both")
-    for p, name, on in ((gamma_post, "gamma_post", post), (beta_post, "beta_post", post),
-                        (gamma_pre, "gamma_pre", pre), (beta_pre, "beta_pre", pre)):
-        if p is None:
-            continue
-        if not on:
-            raise ValueError(f"{name} without its norm")
-        if name.startswith("beta") and norm == "rms":
-            raise ValueError(f"{name}: RMS normalization has no beta")
-        _like(p, cols, torch.float32, name)
+    if not kind and (beta_post is not None or beta_pre is not None):
+        raise ValueError("RMS normalization has no beta")
+    if not post and (gamma_post is not None or beta_post is not None):
+        raise ValueError("gamma_post / beta_post without their norm")
+    if not pre and (gamma_pre is not None or beta_pre is not None):
+        raise ValueError("gamma_pre / beta_pre without their norm")
+    _like(gamma_post, cols, torch.float32, "gamma_post")
+    _like(beta_post, cols, torch.float32, "beta_post")
+    _like(gamma_pre, cols, torch.float32, "gamma_pre")
+    _like(beta_pre, cols, torch.float32, "beta_pre")
 
 
 def resnorm_forward(x, res, outer, gate=None, gamma_post=None, beta_post=None, gamma_pre=None,
@@ -835,41 +837,33 @@ def resnorm_forward(x, res, outer, gate=None, gamma_post=None, beta_post=None, g
     reads.  h may be res, y may be x (in place).  Returns ResNorm."""
     import torch
     rows, cols = _rows_cols(x, outer)
-    dt, kind = _token_dtype(x.dtype), NORMS[norm]
-    layer = kind == 1
-    with _On(x, res, gate, gamma_post, beta_post, gamma_pre, beta_pre, h, y) as st:
-        _like(res, rows * cols, x.dtype, "res")
-        _step_params(cols, post, pre, norm, gamma_post, beta_post, gamma_pre, beta_pre)
-        gk, gr = _gate_args(gate, rows, cols, x.dtype)
-        h = torch.empty_like(x) if h is None else _like(h, rows * cols, x.dtype, "h")
-        if pre:
-            y = torch.empty_like(x) if y is None else _like(y, rows * cols, x.dtype, "y")
-        else:
-            y = None
-        # the statistics in one allocation
-        each = torch.empty(((int(post) + int(pre)) * (1 + kind), rows), dtype=torch.float32,
-                           device=x.device).unbind(0)
-        it = iter(each)
-        stats = [next(it) if on and (layer or k) else None
-                 for on in (post, pre) for k in (0, 1)]
-        x8 = h8 = None
-        f = 0
-        if checkpoint is not None:
-            f = ACT8_FORMATS[checkpoint]
-            qd = torch.int8 if f == 1 else torch.float8_e4m3fn
+    act, dev = x.dtype, x.device
+    dt, kind = _token_dtype(act), NORMS[norm]
+    gpu = _one_gpu(x, res, gate, gamma_post, beta_post, gamma_pre, beta_pre, h, y)
+    _like(res, rows * cols, act, "res")
+    _step_params(cols, post, pre, kind, gamma_post, beta_post, gamma_pre, beta_pre)
+    gk, gr = _gate_args(gate, rows, cols, act)
+    h = torch.empty_like(x) if h is None else _like(h, rows * cols, act, "h")
+    if pre:
+        y = torch.empty_like(x) if y is None else _like(y, rows * cols, act, "y")
+    else:
+        y = None
 
-            def copy():
-                return Act8(torch.empty(x.shape, dtype=qd, device=x.device),
-                            torch.empty((rows, (cols + 31) // 32), dtype=torch.uint8, device=x.device))
-            x8 = copy() if post or gk else None
-            h8 = copy() if pre else None
-        check(lib().nblahip_resnorm_fwd(
-            _ptr(x), _ptr(res), _ptr(gate), gk, gr, _ptr(gamma_post), _ptr(beta_post), _ptr(gamma_pre),
-            _ptr(beta_pre), _ptr(h), _ptr(y), _ptr(stats[0]), _ptr(stats[1]), _ptr(stats[2]),
-            _ptr(stats[3]), _ptr(x8 and x8.codes), _ptr(x8 and x8.scales), _ptr(h8 and h8.codes),
-            _ptr(h8 and h8.scales), f, rows, cols, res_scale, branch_scale, eps, kind, int(post),
-            int(pre), dt, st))
-    return ResNorm(h, y, tuple(stats), x8, h8)
+    def stat(on):
+        return torch.empty(rows, dtype=torch.float32, device=dev) if on else None
+    stats = (stat(post and kind), stat(post), stat(pre and kind), stat(pre))
+    x8 = h8 = None
+    f = 0
+    if checkpoint is not None:
+        f = ACT8_FORMATS[checkpoint]
+        x8 = _new_act8(x, rows, cols, f) if post or gk else None
+        h8 = _new_act8(x, rows, cols, f) if pre else None
+    _call(gpu, lib().nblahip_resnorm_fwd, _ptr(x), _ptr(res), _ptr(gate), gk, gr, _ptr(gamma_post),
+          _ptr(beta_post), _ptr(gamma_pre), _ptr(beta_pre), _ptr(h), _ptr(y), _ptr(stats[0]),
+          _ptr(stats[1]), _ptr(stats[2]), _ptr(stats[3]), _ptr(x8 and x8.codes),
+          _ptr(x8 and x8.scales), _ptr(h8 and h8.codes), _ptr(h8 and h8.scales), f, rows, cols,
+          res_scale, branch_scale, eps, kind, int(post), int(pre), dt)
+    return ResNorm(h, y, stats, x8, h8)
 
 
 def resnorm_backward(x, h, dh, dy, stats, outer, gate=None, gamma_post=None, beta_post=None,
@@ -897,43 +891,39 @@ def resnorm_backward(x, h, dh, dy, stats, outer, gate=None, gamma_post=None, bet
     hd, hs, hf = _check_kept(h, "h", rows, cols, act)
     if x is not None and h is not None and xf != hf:
         raise TypeError("x and h must be kept in the same form")
-    out = ResNormGrads(*([None] * 7)) if out is None else out
-    with _On(lead, dh, dy, xd, xs, hd, hs, gate, gamma_post, beta_post, gamma_pre, beta_pre, *stats,
-             *out, ws) as st:
-        _step_params(cols, post, pre, norm, gamma_post, beta_post, gamma_pre, beta_pre)
-        _like(dh, rows * cols, act, "dh")
-        _like(dy, rows * cols, act, "dy")
-        for s, name in zip(stats, ("mean_post", "var_post", "mean_pre", "var_pre")):
-            _like(s, rows, torch.float32, name)
-        have = (True, has_res, gk != 0, post, post and layer, pre, pre and layer)
-        f32 = torch.float32
-        shapes = ((lead.shape, act), (lead.shape, act),
-                  (None if gate is None else gate.shape, act if gk == 2 else f32),
-                  ((cols,), f32), ((cols,), f32), ((cols,), f32), ((cols,), f32))
-        grads = []
-        mask = 0
-        for i in range(7):
-            t = None
-            if have[i] and need[i]:
-                shape, d = shapes[i]
-                t = out[i]
-                if t is None:
-                    t = torch.empty(shape, dtype=d, device=lead.device)
-                else:
-                    n = 1
-                    for k in shape:
-                        n *= k
-                    _like(t, n, d, ResNormGrads._fields[i])
-                if accum[i]:
-                    mask |= _ACCUM_BITS[i]
-            grads.append(t)
-        if ws is None:
-            ws = _workspace(lib().nblahip_resnorm_bwd_workspace_bytes(
-                rows, cols, gk, gr, kind, int(post), int(pre), dt), lead.device)
-        p = [_ptr(g) for g in grads]
-        check(lib().nblahip_resnorm_bwd(
-            _ptr(xd), _ptr(xs), _ptr(hd), _ptr(hs), xf or hf, _ptr(dh), _ptr(dy), _ptr(gate), gk, gr,
-            _ptr(gamma_post), _ptr(beta_post), _ptr(gamma_pre), _ptr(stats[0]), _ptr(stats[1]),
-            _ptr(stats[2]), _ptr(stats[3]), p[0], p[1], p[2], p[3], p[4], p[5], p[6], mask, rows, cols,
-            res_scale, branch_scale, eps, kind, int(post), int(pre), dt, _ptr(ws), ws.numel(), st))
+    out = (None,) * 7 if out is None else out
+    gpu = _one_gpu(lead, dh, dy, xd, xs, hd, hs, gate, gamma_post, beta_post, gamma_pre, beta_pre,
+                   *stats, *out, ws)
+    _step_params(cols, post, pre, kind, gamma_post, beta_post, gamma_pre, beta_pre)
+    _like(dh, rows * cols, act, "dh")
+    _like(dy, rows * cols, act, "dy")
+    for s, name in zip(stats, ("mean_post", "var_post", "mean_pre", "var_pre")):
+        _like(s, rows, torch.float32, name)
+    dev, f32 = lead.device, torch.float32
+    shape, par = (lead.shape, rows * cols, act), ((cols,), cols, f32)
+    shapes = (shape, shape,
+              None if gate is None else (gate.shape, gate.numel(), act if gk == 2 else f32),
+              par, par, par, par)
+    have = (True, has_res, gk != 0, post, post and layer, pre, pre and layer)
+    grads, mask = [], 0
+    for i in range(7):
+        t = None
+        if have[i] and need[i]:
+            t = out[i]
+            if t is None:
+                t = torch.empty(shapes[i][0], dtype=shapes[i][2], device=dev)
+            else:
+                _like(t, shapes[i][1], shapes[i][2], ResNormGrads._fields[i])
+            if accum[i]:
+                mask |= _ACCUM_BITS[i]
+        grads.append(t)
+    if ws is None:
+        ws = _workspace(lib().nblahip_resnorm_bwd_workspace_bytes(
+            rows, cols, gk, gr, kind, int(post), int(pre), dt), dev)
+    p = [_ptr(g) for g in grads]
+    _call(gpu, lib().nblahip_resnorm_bwd, _ptr(xd), _ptr(xs), _ptr(hd), _ptr(hs), xf or hf, _ptr(dh),
+          _ptr(dy), _ptr(gate), gk, gr, _ptr(gamma_post), _ptr(beta_post), _ptr(gamma_pre),
+          _ptr(stats[0]), _ptr(stats[1]), _ptr(stats[2]), _ptr(stats[3]), p[0], p[1], p[2], p[3], p[4],
+          p[5], p[6], mask, rows, cols, res_scale, branch_scale, eps, kind, int(post), int(pre), dt,
+          _ptr(ws), ws.nbytes)
     return ResNormGrads(*grads)

@@ -57,11 +57,13 @@ struct StepPlan {
 // Threads per row of the kernels that keep a row in registers, a 16-byte vector
 // each.
 #define NBLAHIP_STEP_LAYOUTS(CASE) \
-  CASE(16) CASE(32) CASE(64) CASE(128) CASE(256) CASE(512) CASE(1024)
+  CASE(16) CASE(32) CASE(64) CASE(128) CASE(192) CASE(256) CASE(384) CASE(512) CASE(768) CASE(1024)
 
-// Rows a block works on at a time, and its threads.
-inline int step_rows_per_block(int tpr) { return tpr > 0 && tpr < 256 ? 256 / tpr : 1; }
-inline int step_block(int tpr) { return tpr < 256 ? 256 : tpr; }
+// Threads of a block.  Backward: 512 where a row takes 256 or fewer, so that the
+// rows of a block share one partial sum per column (half the partial sums of
+// blocks of 256 at the same number of threads on the chip).
+constexpr int fwd_block(int tpr) { return tpr == 192 ? 192 : tpr < 256 ? 256 : tpr; }
+constexpr int bwd_block(int tpr) { return tpr == 192 ? 384 : tpr < 512 && tpr != 384 ? 512 : tpr; }
 
 int launch_step_fwd_f32(const StepPlan &pl, const StepArgs &a, hipStream_t st);
 int launch_step_fwd_f16(const StepPlan &pl, const StepArgs &a, hipStream_t st);

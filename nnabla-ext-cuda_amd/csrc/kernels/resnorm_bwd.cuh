@@ -12,14 +12,14 @@ template <typename T, bool LN, bool POST, bool PRE, bool Q8, bool ANY>
 bool launch_bwd_rows(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
   // the one form that does not fit the registers of a block of 1024
   // (step_bwd_is_long keeps it away)
-  constexpr int MOST = LN && POST && PRE && Q8 && ANY && sizeof(T) == 2 ? 512 : 1024;
+  constexpr int MOST = LN && POST && PRE && Q8 && ANY && sizeof(T) == 2 ? 768 : 1024;
   switch (pl.tpr) {
 #define NBLAHIP_CASE(TPR)                                                                         \
   case TPR:                                                                                       \
     if constexpr (TPR <= MOST) {                                                                  \
       NBLAHIP_LAUNCH("step_bwd_rows_kernel",                                                      \
                      (step_bwd_rows_kernel<T, LN, POST, PRE, Q8, ANY, TPR>),                      \
-                     dim3(static_cast<unsigned>(a.grid)), dim3(row_block<TPR>()), 0, st, a);      \
+                     dim3(static_cast<unsigned>(a.grid)), dim3(bwd_block(TPR)), 0, st, a);      \
       return true;                                                                                \
     } else {                                                                                      \
       return false;                                                                               \
@@ -32,9 +32,11 @@ bool launch_bwd_rows(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
 
 template <typename T, bool LN, bool POST, bool PRE, bool Q8>
 int launch_bwd_kind(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
-  if (pl.any ? launch_bwd_rows<T, LN, POST, PRE, Q8, true>(pl, a, st)
-             : launch_bwd_rows<T, LN, POST, PRE, Q8, false>(pl, a, st))
-    return last_launch_status();
+  if (pl.tpr != 0) {
+    const bool known = pl.any ? launch_bwd_rows<T, LN, POST, PRE, Q8, true>(pl, a, st)
+                              : launch_bwd_rows<T, LN, POST, PRE, Q8, false>(pl, a, st);
+    return known ? last_launch_status() : NBLAHIP_EINVAL; // (the workspace is not the long rows')
+  }
   const dim3 rows(static_cast<unsigned>(std::min<int64_t>(a.rows, 1 << 20)));
   NBLAHIP_LAUNCH("step_bwd_long_sums_kernel", (step_bwd_long_sums_kernel<T, LN, POST, PRE, Q8>), rows,
                  dim3(kLongThreads), 0, st, a);

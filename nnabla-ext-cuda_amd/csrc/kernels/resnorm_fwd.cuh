@@ -14,7 +14,7 @@ bool launch_fwd_rows(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
   case TPR:                                                                                       \
     NBLAHIP_LAUNCH("step_fwd_rows_kernel",                                                        \
                    (step_fwd_rows_kernel<T, LN, POST, PRE, COPY, ANY, TPR>),                      \
-                   dim3(static_cast<unsigned>(a.grid)), dim3(row_block<TPR>()), 0, st, a);        \
+                   dim3(static_cast<unsigned>(a.grid)), dim3(fwd_block(TPR)), 0, st, a);        \
     return true;
     NBLAHIP_STEP_LAYOUTS(NBLAHIP_CASE)
 #undef NBLAHIP_CASE
@@ -25,12 +25,14 @@ bool launch_fwd_rows(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
 template <typename T, bool LN, bool POST, bool PRE>
 int launch_fwd_kind(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
   const bool copy = a.x8 || a.h8;
-  const bool done =
-      pl.any ? copy ? launch_fwd_rows<T, LN, POST, PRE, true, true>(pl, a, st)
-                    : launch_fwd_rows<T, LN, POST, PRE, false, true>(pl, a, st)
-             : copy ? launch_fwd_rows<T, LN, POST, PRE, true, false>(pl, a, st)
-                    : launch_fwd_rows<T, LN, POST, PRE, false, false>(pl, a, st);
-  if (done) return last_launch_status();
+  if (pl.tpr != 0) {
+    const bool known =
+        pl.any ? copy ? launch_fwd_rows<T, LN, POST, PRE, true, true>(pl, a, st)
+                      : launch_fwd_rows<T, LN, POST, PRE, false, true>(pl, a, st)
+               : copy ? launch_fwd_rows<T, LN, POST, PRE, true, false>(pl, a, st)
+                      : launch_fwd_rows<T, LN, POST, PRE, false, false>(pl, a, st);
+    return known ? last_launch_status() : NBLAHIP_EINVAL;
+  }
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(a.rows, 1 << 20)));
   NBLAHIP_LAUNCH("step_fwd_long_kernel", (step_fwd_long_kernel<T, LN, POST, PRE>), grid,
                  dim3(kLongThreads), 0, st, a);

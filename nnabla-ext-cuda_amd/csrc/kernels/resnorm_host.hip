@@ -64,13 +64,16 @@ constexpr int kCus = 256;
 
 int vec_of(int dtype) { return dtype == NBLAHIP_F32 ? 4 : 8; }
 
-// As many threads as the row has vectors, up to a block of 1024; longer rows,
+// The layout with just enough threads for the row's vectors; longer rows,
 // and those of less than a vector, go to the kernels for long rows.
 void pick_layout(StepPlan &pl, int64_t cols) {
   const int64_t vec = vec_of(pl.dtype), vectors = (cols + vec - 1) / vec;
-  pl.tpr = 16;
-  while (pl.tpr < 1024 && pl.tpr < vectors) pl.tpr *= 2;
-  if (pl.tpr < vectors || cols < vec) pl.tpr = 0;
+  pl.tpr = 0;
+  if (cols < vec) return;
+#define NBLAHIP_CASE(TPR) \
+  if (pl.tpr == 0 && vectors <= TPR) pl.tpr = TPR;
+  NBLAHIP_STEP_LAYOUTS(NBLAHIP_CASE)
+#undef NBLAHIP_CASE
 }
 
 // Whether every address that a 16-byte vector of the tensors (or its 8-bit
@@ -116,8 +119,9 @@ size_t plan_bwd(StepArgs &a, StepPlan &pl, int64_t gate_rows, char *ws) {
     plan_chunks(a, gate_rows, kCus, 16);
     a.grid = static_cast<int>(std::min<int64_t>(a.chunks, 1 << 30));
   } else {
-    const int64_t blocks = kCus * std::max<int64_t>(1, 1024 / step_block(pl.tpr));
-    plan_chunks(a, gate_rows, blocks, step_rows_per_block(pl.tpr));
+    const int block = bwd_block(pl.tpr);
+    const int64_t blocks = kCus * std::max(1, 1024 / block);
+    plan_chunks(a, gate_rows, blocks, block / pl.tpr);
     a.grid = static_cast<int>(std::min<int64_t>(a.chunks, blocks));
   }
   size_t at = 0;
@@ -134,11 +138,13 @@ size_t plan_bwd(StepArgs &a, StepPlan &pl, int64_t gate_rows, char *ws) {
 }
 
 // ---------------------------------------------------------------------------
-// Column sums of the partial sums.  16 lanes of 4 columns by 16 rows of threads;
-// blockIdx.y: 0 the second norm's parameters, 1 the first norm's (a shared
-// gate's rows multiplied in), 2 + g gate row g.  The order of the additions is
-// fixed by the sizes.
+// Column sums of the partial sums.  A block takes 32 columns (128 bytes of each
+// partial row): 8 threads of 4 columns by 64 rows.  blockIdx.y: 0 / 1 the second
+// norm's gamma / beta, 2 / 3 the first norm's (a shared gate's rows multiplied
+// in), 4 + g gate row g.  The order of the additions is fixed by the sizes.
 // ---------------------------------------------------------------------------
+constexpr int kFoldLanes = 8, kFoldRows = 64;
+
 struct FoldArgs {
   const float *part_pre, *part_post, *gate, *gamma_post, *beta_post;
   float *dgamma_pre, *dbeta_pre, *dgamma_post, *dbeta_post, *dgate;
@@ -146,18 +152,21 @@ struct FoldArgs {
   unsigned accum;
   int sums;      // 1 or 2 sums per partial row
   int post;      // whether dgate goes through the first norm's parameters
-  int want_pre, want_post;
 };
 
 __device__ __forceinline__ float4 add4(float4 a, float4 b) {
   return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
 }
 
-__device__ __forceinline__ void fold_rows(const float *p, int64_t n, int64_t stride,
-                                          const float *weight, int64_t per, int64_t cols, int64_t c,
-                                          int nc, float4 &s) {
-  const int lane = threadIdx.x / 16;
-  for (int64_t r = lane; r < n; r += 16) {
+// Sum of n rows at p, `stride` floats apart, at the block's columns; the first
+// 8 threads have it.  weight: row r counts times row r / per of it.
+__device__ __forceinline__ float4 fold_rows(const float *p, int64_t n, int64_t stride,
+                                            const float *weight, int64_t per, int64_t cols, int64_t c,
+                                            int nc, float4 *lds) {
+  const int row = threadIdx.x / kFoldLanes, lane = threadIdx.x % kFoldLanes;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int64_t r = row; r < n; r += kFoldRows) {
     float4 v = *reinterpret_cast<const float4 *>(p + r * stride + c);
     if (weight) {
       float w[4];
@@ -166,76 +175,63 @@ __device__ __forceinline__ void fold_rows(const float *p, int64_t n, int64_t str
     }
     s = add4(s, v);
   }
-}
-
-__device__ __forceinline__ float4 fold_block(float4 v, float4 *lds) {
   __syncthreads();
-  lds[threadIdx.x] = v;
+  lds[threadIdx.x] = s;
   __syncthreads();
-  float4 s = lds[threadIdx.x & 15];
-  for (int i = 1; i < 16; ++i) s = add4(s, lds[i * 16 + (threadIdx.x & 15)]);
+  if (row < 8) {
+    for (int i = 1; i < 8; ++i) s = add4(s, lds[(row + 8 * i) * kFoldLanes + lane]);
+  }
+  __syncthreads();
+  if (row < 8) lds[threadIdx.x] = s;
+  __syncthreads();
+  if (row == 0) {
+    for (int i = 1; i < 8; ++i) s = add4(s, lds[i * kFoldLanes + lane]);
+  }
   return s;
 }
 
 __device__ __forceinline__ void fold_put(float *out, int64_t c, int nc, float4 v, bool add) {
-  if (!out || threadIdx.x >= 16) return;
+  if (threadIdx.x >= kFoldLanes) return;
   const float o[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     if (j < nc) out[c + j] = add ? out[c + j] + o[j] : o[j];
 }
 
-__global__ __launch_bounds__(256) void step_fold_kernel(const FoldArgs a) {
-  __shared__ float4 lds[256];
-  const int64_t c = (static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x & 15)) * 4;
+__global__ __launch_bounds__(kFoldLanes *kFoldRows) void step_fold_kernel(const FoldArgs a) {
+  __shared__ float4 lds[kFoldLanes * kFoldRows];
+  const int64_t c = (static_cast<int64_t>(blockIdx.x) * kFoldLanes + threadIdx.x % kFoldLanes) * 4;
   const int64_t cs = least(c, a.pitch - 4); // threads beyond the columns read the last ones
   const int nc = columns_left(a.cols - c, 4);
-  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
   const int64_t stride = a.sums * a.pitch;
-  if (blockIdx.y == 0) {
-    if (!a.want_pre) return;
-    float4 s = zero, t = zero;
-    fold_rows(a.part_pre, a.n_pre, stride, nullptr, 1, a.cols, cs, nc, s);
-    s = fold_block(s, lds);
-    fold_put(a.dgamma_pre, c, nc, s, a.accum & NBLAHIP_ACCUM_DGAMMA_PRE);
-    if (a.sums == 2 && a.dbeta_pre) {
-      fold_rows(a.part_pre + a.pitch, a.n_pre, stride, nullptr, 1, a.cols, cs, nc, t);
-      t = fold_block(t, lds);
-      fold_put(a.dbeta_pre, c, nc, t, a.accum & NBLAHIP_ACCUM_DBETA_PRE);
-    }
-  } else if (blockIdx.y == 1) {
-    if (!a.want_post) return;
-    float4 s = zero, t = zero;
-    fold_rows(a.part_post, a.chunks, stride, a.gate, a.chunks_per_gate, a.cols, cs, nc, s);
-    s = fold_block(s, lds);
-    fold_put(a.dgamma_post, c, nc, s, a.accum & NBLAHIP_ACCUM_DGAMMA_POST);
-    if (a.sums == 2 && a.dbeta_post) {
-      fold_rows(a.part_post + a.pitch, a.chunks, stride, a.gate, a.chunks_per_gate, a.cols, cs, nc, t);
-      t = fold_block(t, lds);
-      fold_put(a.dbeta_post, c, nc, t, a.accum & NBLAHIP_ACCUM_DBETA_POST);
-    }
-  } else {
-    for (int64_t g = blockIdx.y - 2; g < a.gate_rows; g += gridDim.y - 2) {
-      float4 s = zero;
-      const float *p = a.part_post + g * a.chunks_per_gate * stride;
-      const int64_t n = a.chunks > 0 ? a.chunks_per_gate : 0;
-      fold_rows(p, n, stride, nullptr, 1, a.cols, cs, nc, s);
-      s = fold_block(s, lds);
-      if (a.post) {
-        float ga[4], be[4];
-        load_param<4>(a.gamma_post, c, nc, ga);
+  if (blockIdx.y < 4) {
+    const bool beta = blockIdx.y & 1, first = blockIdx.y >= 2;
+    float *out = first ? (beta ? a.dbeta_post : a.dgamma_post) : (beta ? a.dbeta_pre : a.dgamma_pre);
+    if (!out) return;
+    const float *p = (first ? a.part_post : a.part_pre) + (beta ? a.pitch : 0);
+    const float4 s = fold_rows(p, first ? a.chunks : a.n_pre, stride, first ? a.gate : nullptr,
+                               a.chunks_per_gate, a.cols, cs, nc, lds);
+    fold_put(out, c, nc, s,
+             a.accum & (first ? (beta ? NBLAHIP_ACCUM_DBETA_POST : NBLAHIP_ACCUM_DGAMMA_POST)
+                              : (beta ? NBLAHIP_ACCUM_DBETA_PRE : NBLAHIP_ACCUM_DGAMMA_PRE)));
+    return;
+  }
+  for (int64_t g = blockIdx.y - 4; g < a.gate_rows; g += gridDim.y - 4) {
+    const float *p = a.part_post + g * a.chunks_per_gate * stride;
+    const int64_t n = a.chunks > 0 ? a.chunks_per_gate : 0;
+    float4 s = fold_rows(p, n, stride, nullptr, 1, a.cols, cs, nc, lds);
+    if (a.post) {
+      float ga[4], be[4];
+      load_param<4>(a.gamma_post, c, nc, ga);
+      s.x *= ga[0]; s.y *= ga[1]; s.z *= ga[2]; s.w *= ga[3];
+      if (a.sums == 2 && a.beta_post) {
         load_bias<4>(a.beta_post, c, nc, be);
-        s.x *= ga[0]; s.y *= ga[1]; s.z *= ga[2]; s.w *= ga[3];
-        if (a.sums == 2 && a.beta_post) {
-          float4 t = zero;
-          fold_rows(p + a.pitch, n, stride, nullptr, 1, a.cols, cs, nc, t);
-          t = fold_block(t, lds);
-          s.x = fmaf(t.x, be[0], s.x); s.y = fmaf(t.y, be[1], s.y);
-          s.z = fmaf(t.z, be[2], s.z); s.w = fmaf(t.w, be[3], s.w);
-        }
+        const float4 t = fold_rows(p + a.pitch, n, stride, nullptr, 1, a.cols, cs, nc, lds);
+        s.x = fmaf(t.x, be[0], s.x); s.y = fmaf(t.y, be[1], s.y);
+        s.z = fmaf(t.z, be[2], s.z); s.w = fmaf(t.w, be[3], s.w);
       }
-      fold_put(a.dgate + g * a.cols, c, nc, s, a.accum & NBLAHIP_ACCUM_DGATE);
     }
+    fold_put(a.dgate + g * a.cols, c, nc, s, a.accum & NBLAHIP_ACCUM_DGATE);
   }
 }
 
@@ -244,15 +240,13 @@ int launch_fold(const StepArgs &a, const StepPlan &pl, int64_t gate_rows, hipStr
   const bool shared = a.gate_kind == NBLAHIP_GATE_ROWS;
   f.part_pre = a.part_pre;
   f.part_post = a.part_post;
-  f.want_pre = pl.pre && (a.dgamma_pre || a.dbeta_pre);
-  f.want_post = pl.post && (a.dgamma_post || a.dbeta_post);
   f.gate = shared ? static_cast<const float *>(a.gate) : nullptr;
   f.gamma_post = a.gamma_post;
   f.beta_post = a.beta_post;
-  f.dgamma_pre = a.dgamma_pre;
-  f.dbeta_pre = a.dbeta_pre;
-  f.dgamma_post = a.dgamma_post;
-  f.dbeta_post = a.dbeta_post;
+  f.dgamma_pre = pl.pre ? a.dgamma_pre : nullptr;
+  f.dbeta_pre = pl.pre && pl.layer ? a.dbeta_pre : nullptr;
+  f.dgamma_post = pl.post ? a.dgamma_post : nullptr;
+  f.dbeta_post = pl.post && pl.layer ? a.dbeta_post : nullptr;
   f.dgate = shared ? static_cast<float *>(a.dgate) : nullptr;
   f.n_pre = a.chunks > 0 ? a.grid : 0;
   f.chunks = a.chunks;
@@ -263,10 +257,11 @@ int launch_fold(const StepArgs &a, const StepPlan &pl, int64_t gate_rows, hipStr
   f.accum = a.accum;
   f.sums = pl.layer ? 2 : 1;
   f.post = pl.post;
-  if (!f.want_pre && !f.want_post && !f.dgate) return 0;
-  const int64_t ny = 2 + std::min<int64_t>(f.gate_rows, kGridY - 2);
-  const dim3 grid(static_cast<unsigned>((a.cols + 63) / 64), static_cast<unsigned>(ny));
-  NBLAHIP_LAUNCH("step_fold_kernel", step_fold_kernel, grid, dim3(256), 0, st, f);
+  if (!f.dgamma_pre && !f.dbeta_pre && !f.dgamma_post && !f.dbeta_post && !f.dgate) return 0;
+  const int64_t ny = 4 + std::min<int64_t>(f.gate_rows, kGridY - 4);
+  const int span = 4 * kFoldLanes;
+  const dim3 grid(static_cast<unsigned>((a.cols + span - 1) / span), static_cast<unsigned>(ny));
+  NBLAHIP_LAUNCH("step_fold_kernel", step_fold_kernel, grid, dim3(kFoldLanes * kFoldRows), 0, st, f);
   return last_launch_status();
 }
 
@@ -315,8 +310,9 @@ int step_fwd(StepArgs a, StepPlan pl, int64_t gate_rows, hipStream_t st) {
   pl.any = a.gate_kind == NBLAHIP_GATE_FULL ||
            !whole_vectors(pl.dtype, a.cols, {a.x, a.res, a.h, a.y}, {a.x8, a.h8});
   gate_rows = shared_gate_rows(a, gate_rows);
-  const int64_t blocks = kCus * (2048 / step_block(pl.tpr));
-  plan_chunks(a, gate_rows, blocks, step_rows_per_block(pl.tpr));
+  const int block = pl.tpr ? fwd_block(pl.tpr) : 1024;
+  const int64_t blocks = kCus * (2048 / block);
+  plan_chunks(a, gate_rows, blocks, pl.tpr ? block / pl.tpr : 1);
   a.grid = static_cast<int>(std::min<int64_t>(a.chunks, blocks));
   return run_fwd(pl, a, st);
 }

@@ -1,8 +1,8 @@
 // The residual step on rows that fit a block at one 16-byte vector per thread:
 // every tensor crosses HBM once per direction.
 //
-// TPR threads hold a row; blocks of 256 threads take several rows at a time
-// where TPR < 256.  A thread's columns are the same in every row, so the
+// TPR threads hold a row; a block takes several rows at a time where they are
+// short.  A thread's columns are the same in every row, so the
 // parameters (and, backward, the column sums of the parameter gradients) stay
 // in its registers while the block walks its rows.
 //
@@ -32,10 +32,8 @@ namespace nblahip {
 // sums.  Rows of several waves go through LDS: two buffers taken in turn, so
 // that one barrier per sum is enough (a wave writes a buffer again only after
 // the barrier of the sum in between, which every wave reaches after its reads).
-template <int TPR, int N> struct RowTotal {
-  static constexpr int kWaves = TPR > kWave ? TPR / kWave : 1;
-  static constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
-  static constexpr int kFloats = TPR > kWave ? 2 * kRows * kWaves * N : 1;
+template <int TPR, int BLOCK, int N> struct RowTotal {
+  static constexpr int kFloats = TPR > kWave ? 2 * (BLOCK / kWave) * N : 2;
 };
 
 template <int TPR, int N, int CAP>
@@ -68,7 +66,6 @@ __device__ __forceinline__ void row_total(float (&v)[N], float (&lds)[CAP], int 
   }
 }
 
-template <int TPR> constexpr int row_block() { return TPR < 256 ? 256 : TPR; }
 
 typedef __amdgpu_buffer_rsrc_t Buffer;
 constexpr uint32_t kOutside = 0x7fffffffu; // an offset past every buffer here
@@ -120,16 +117,15 @@ template <int N> __device__ __forceinline__ void settle(float (&v)[N]) {
 // the first of them: of a tensor of the storage type, of 8-bit codes, of their
 // scales, of a row statistic.  With ANY the thread a row ends in reads the
 // vector `drop` elements further ahead, and writes the first `n` of its own.
-template <typename T, int TPR, bool ANY> struct Place {
+template <typename T, int TPR, int BLOCK, bool ANY> struct Place {
   static constexpr int V = Tok<T>::VEC;
-  static constexpr int RPB = row_block<TPR>() / TPR;
   static constexpr uint32_t SZ = sizeof(T);
   uint32_t wide, codes, scale, stat;
   uint32_t drop; // ANY only
   int c, n;      // the thread's first column, and how many it has
   __device__ __forceinline__ Place(const StepArgs &a) {
     const uint32_t cols = static_cast<uint32_t>(a.cols);
-    const uint32_t sub = TPR >= 256 ? 0 : threadIdx.x / TPR;
+    const uint32_t sub = BLOCK == TPR ? 0 : threadIdx.x / TPR;
     c = (threadIdx.x % TPR) * V;
     n = columns_left(a.cols - c, V);
     drop = ANY && n > 0 ? V - n : 0;
@@ -244,12 +240,12 @@ template <int RPB> __device__ __forceinline__ uint32_t rows_in(int64_t base, int
 
 // Forward.  A block takes runs of rows (chunks) that share a gate row.
 template <typename T, bool LN, bool POST, bool PRE, bool COPY, bool ANY, int TPR>
-__global__ __launch_bounds__(row_block<TPR>()) void step_fwd_rows_kernel(const StepArgs a) {
+__global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const StepArgs a) {
   constexpr int V = Tok<T>::VEC;
-  constexpr int RPB = row_block<TPR>() / TPR;
-  __shared__ float lds[RowTotal<TPR, 1>::kFloats < 2 ? 2 : RowTotal<TPR, 1>::kFloats];
+  constexpr int BLOCK = fwd_block(TPR), RPB = BLOCK / TPR;
+  __shared__ float lds[RowTotal<TPR, BLOCK, 1>::kFloats];
   int turn = 0;
-  const Place<T, TPR, ANY> pl(a);
+  const Place<T, TPR, BLOCK, ANY> pl(a);
   const uint32_t row_bytes = static_cast<uint32_t>(a.cols) * static_cast<uint32_t>(sizeof(T));
   const float inv = 1.f / static_cast<float>(a.cols);
   const uint32_t stat_out = threadIdx.x % TPR == 0 ? pl.stat : kOutside;
@@ -365,10 +361,10 @@ __global__ __launch_bounds__(row_block<TPR>()) void step_fwd_rows_kernel(const S
 }
 
 // A kept tensor's vector as it was loaded: storage type, or an 8-bit copy.
-template <typename T, bool Q8, int TPR, bool ANY> struct Kept {
+template <typename T, bool Q8, int TPR, int BLOCK, bool ANY> struct Kept {
   Packed p;
   __device__ __forceinline__ void ask(const StepArgs &a, const void *data, const uint8_t *, int64_t base,
-                                      uint32_t rows, const Place<T, TPR, ANY> &pl) {
+                                      uint32_t rows, const Place<T, TPR, BLOCK, ANY> &pl) {
     p = pl.load(buffer(data, base * a.cols * static_cast<int64_t>(sizeof(T)),
                        rows * static_cast<uint32_t>(a.cols) * static_cast<uint32_t>(sizeof(T))));
   }
@@ -381,11 +377,11 @@ template <typename T, bool Q8, int TPR, bool ANY> struct Kept {
     if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(p.v.x), "+v"(p.v.y), "+v"(p.v.z), "+v"(p.v.w));
   }
 };
-template <typename T, int TPR, bool ANY> struct Kept<T, true, TPR, ANY> {
+template <typename T, int TPR, int BLOCK, bool ANY> struct Kept<T, true, TPR, BLOCK, ANY> {
   uint2 q;
   uint32_t code;
   __device__ __forceinline__ void ask(const StepArgs &a, const void *data, const uint8_t *scales,
-                                      int64_t base, uint32_t rows, const Place<T, TPR, ANY> &pl) {
+                                      int64_t base, uint32_t rows, const Place<T, TPR, BLOCK, ANY> &pl) {
     q = pl.load_codes(buffer(data, base * a.cols, rows * static_cast<uint32_t>(a.cols)));
     code = __builtin_amdgcn_raw_buffer_load_b8(
         buffer(scales, base * a.groups8, rows * static_cast<uint32_t>(a.groups8)), pl.scale, 0, 0);
@@ -444,14 +440,14 @@ template <int V, int TPR> struct ColumnSum<V, TPR, true> {
 // Backward.  Each input vector is asked for again, for the next row, right
 // after its last use.
 template <typename T, bool LN, bool POST, bool PRE, bool Q8, bool ANY, int TPR>
-__global__ __launch_bounds__(row_block<TPR>()) void step_bwd_rows_kernel(const StepArgs a) {
+__global__ __launch_bounds__(bwd_block(TPR)) void step_bwd_rows_kernel(const StepArgs a) {
   constexpr int V = Tok<T>::VEC;
-  constexpr int RPB = row_block<TPR>() / TPR;
+  constexpr int BLOCK = bwd_block(TPR), RPB = BLOCK / TPR;
   constexpr int S = LN ? 2 : 1; // row sums per norm, column sums per norm
-  __shared__ float lds[RowTotal<TPR, S>::kFloats < 2 ? 2 : RowTotal<TPR, S>::kFloats];
-  __shared__ float fold[RPB > 1 ? 256 * V : 1];
+  __shared__ float lds[RowTotal<TPR, BLOCK, S>::kFloats];
+  __shared__ float fold[RPB > 1 ? BLOCK * V : 1];
   int turn = 0;
-  const Place<T, TPR, ANY> pl(a);
+  const Place<T, TPR, BLOCK, ANY> pl(a);
   const uint32_t row_bytes = static_cast<uint32_t>(a.cols) * static_cast<uint32_t>(sizeof(T));
   const float inv = 1.f / static_cast<float>(a.cols);
   float kp[V], gn[V];
@@ -470,7 +466,7 @@ __global__ __launch_bounds__(row_block<TPR>()) void step_bwd_rows_kernel(const S
   C.clear(c_lds);
   E.clear(e_lds);
 
-  Kept<T, Q8, TPR, ANY> x, h;
+  Kept<T, Q8, TPR, BLOCK, ANY> x, h;
   Packed dh, dy, gf;
   float m1 = 0.f, v1 = 0.f, m2 = 0.f, v2 = 0.f;
   // Column sums (times `scale`) of the block's rows-at-a-time to `out`; every
@@ -486,14 +482,14 @@ __global__ __launch_bounds__(row_block<TPR>()) void step_bwd_rows_kernel(const S
     } else {
       lds_barrier();
 #pragma unroll
-      for (int j = 0; j < V; ++j) fold[j * 256 + threadIdx.x] = s[j];
+      for (int j = 0; j < V; ++j) fold[j * BLOCK + threadIdx.x] = s[j];
       lds_barrier();
-      // 256 threads over the TPR * V columns of the tile, RPB values each
-      for (int i = threadIdx.x; i < TPR * V; i += 256) {
+      // the block over the TPR * V columns of the tile, RPB values each
+      for (int i = threadIdx.x; i < TPR * V; i += BLOCK) {
         const int j = i / TPR, l = i % TPR;
         float t = 0.f;
 #pragma unroll
-        for (int q = 0; q < RPB; ++q) t += fold[j * 256 + q * TPR + l];
+        for (int q = 0; q < RPB; ++q) t += fold[j * BLOCK + q * TPR + l];
         if (l * V + j < a.pitch) out[l * V + j] = t * scale;
       }
     }
