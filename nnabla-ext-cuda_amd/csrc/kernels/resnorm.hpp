@@ -57,13 +57,37 @@ struct StepPlan {
 // Threads per row of the kernels that keep a row in registers, a 16-byte vector
 // each.
 #define NBLAHIP_STEP_LAYOUTS(CASE) \
-  CASE(16) CASE(32) CASE(64) CASE(128) CASE(192) CASE(256) CASE(384) CASE(512) CASE(768) CASE(1024)
+  CASE(16) CASE(32) CASE(64) CASE(128) CASE(192) CASE(256) CASE(384) CASE(512) CASE(640) CASE(768) CASE(1024)
 
 // Threads of a block.  Backward: 512 where a row takes 256 or fewer, so that the
 // rows of a block share one partial sum per column (half the partial sums of
 // blocks of 256 at the same number of threads on the chip).
 constexpr int fwd_block(int tpr) { return tpr == 192 ? 192 : tpr < 256 ? 256 : tpr; }
 constexpr int bwd_block(int tpr) { return tpr == 192 ? 384 : tpr < 512 && tpr != 384 ? 512 : tpr; }
+
+// Backward: waves per SIMD that the registers of the row kernels allow (what the
+// compiler needs without a limit: 56 - 119 registers a thread, 76 - 148 with
+// `any`), and from them how many blocks a CU has at once: as many as are
+// launched, each walking its share of the rows.
+constexpr int bwd_waves(int vec, bool layer, bool post, bool pre, bool any, int tpr) {
+  if (tpr == 1024) return 4;
+  if (vec == 4) return any && layer && post && pre ? 4 : any || (layer && post && pre) ? 5 : 6;
+  if (layer) return (post && pre ? 4 : pre ? 4 : 5) - (any ? 1 : 0);
+  return (pre ? 5 : 6) - (any ? (pre ? 1 : 2) : 0);
+}
+constexpr int bwd_blocks_per_cu(int vec, bool layer, bool post, bool pre, bool any, int tpr) {
+  const int n = 256 * bwd_waves(vec, layer, post, pre, any, tpr) / bwd_block(tpr);
+  return n > 0 ? n : 1;
+}
+// Rows whose loads are in flight ahead of the one in hand: two where a CU has one
+// block, which otherwise stands still while its next row arrives ([8192, 8192]
+// bf16 175 -> 158 us; more blocks per CU do not gain), unless the registers of
+// a block of 1024 are full.
+constexpr int bwd_depth(int vec, bool layer, bool post, bool pre, bool any, int tpr) {
+  const bool full = tpr == 1024 && (vec == 8 ? any || (layer && post && pre) : any && layer);
+  return bwd_blocks_per_cu(vec, layer, post, pre, any, tpr) == 1 && !full ? 2 : 1;
+}
+constexpr int fwd_depth(int tpr, bool any) { return tpr >= 256 && !(any && tpr == 1024) ? 2 : 1; }
 
 int launch_step_fwd_f32(const StepPlan &pl, const StepArgs &a, hipStream_t st);
 int launch_step_fwd_f16(const StepPlan &pl, const StepArgs &a, hipStream_t st);

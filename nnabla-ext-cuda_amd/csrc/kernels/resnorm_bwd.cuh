@@ -12,7 +12,7 @@ template <typename T, bool LN, bool POST, bool PRE, bool Q8, bool ANY>
 bool launch_bwd_rows(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
   // the one form that does not fit the registers of a block of 1024
   // (step_bwd_is_long keeps it away)
-  constexpr int MOST = LN && POST && PRE && Q8 && ANY && sizeof(T) == 2 ? 768 : 1024;
+  constexpr int MOST = LN && POST && PRE && ANY && sizeof(T) == 2 ? 768 : 1024;
   switch (pl.tpr) {
 #define NBLAHIP_CASE(TPR)                                                                         \
   case TPR:                                                                                       \

@@ -106,21 +106,21 @@ int64_t shared_gate_rows(const StepArgs &a, int64_t gate_rows) {
 }
 
 // The backward's only form whose rows of 1024 threads do not fit the registers.
-bool step_bwd_is_long(const StepPlan &pl, bool any, bool kept8) {
-  return pl.tpr == 1024 && pl.dtype != NBLAHIP_F32 && pl.layer && pl.post && pl.pre && any && kept8;
+bool step_bwd_is_long(const StepPlan &pl) {
+  return pl.tpr == 1024 && pl.dtype != NBLAHIP_F32 && pl.layer && pl.post && pl.pre && pl.any;
 }
 
 // The backward's split, and its workspace laid out from `ws` (null: sizes only).
 size_t plan_bwd(StepArgs &a, StepPlan &pl, int64_t gate_rows, char *ws) {
   pick_layout(pl, a.cols);
-  if (step_bwd_is_long(pl, pl.any, pl.kept8)) pl.tpr = 0;
+  if (step_bwd_is_long(pl)) pl.tpr = 0;
   a.pitch = (a.cols + 7) / 8 * 8;
   if (pl.tpr == 0) {
     plan_chunks(a, gate_rows, kCus, 16);
     a.grid = static_cast<int>(std::min<int64_t>(a.chunks, 1 << 30));
   } else {
     const int block = bwd_block(pl.tpr);
-    const int64_t blocks = kCus * std::max(1, 1024 / block);
+    const int64_t blocks = kCus * bwd_blocks_per_cu(vec_of(pl.dtype), pl.layer, pl.post, pl.pre, pl.any, pl.tpr);
     plan_chunks(a, gate_rows, blocks, block / pl.tpr);
     a.grid = static_cast<int>(std::min<int64_t>(a.chunks, blocks));
   }
@@ -522,10 +522,14 @@ size_t nblahip_resnorm_bwd_workspace_bytes(int64_t rows, int64_t cols, int gate_
   a.cols = cols;
   a.gate_kind = gate_kind;
   const int64_t g = shared_gate_rows(a, gate_rows);
-  StepArgs b = a;
-  StepPlan ql = pl;
-  ql.any = ql.kept8 = true; // the call may be of the form that runs as a long row
-  return std::max(plan_bwd(a, pl, g, nullptr), plan_bwd(b, ql, g, nullptr));
+  size_t most = 0; // over the forms a call of these sizes may take
+  for (const bool any : {false, true}) {
+    StepArgs b = a;
+    StepPlan q = pl;
+    q.any = any;
+    most = std::max(most, plan_bwd(b, q, g, nullptr));
+  }
+  return most;
 }
 
 int nblahip_resnorm_bwd(const void *x, const uint8_t *x_scale, const void *h, const uint8_t *h_scale,

@@ -69,13 +69,16 @@ __device__ __forceinline__ void row_total(float (&v)[N], float (&lds)[CAP], int 
 
 typedef __amdgpu_buffer_rsrc_t Buffer;
 constexpr uint32_t kOutside = 0x7fffffffu; // an offset past every buffer here
-constexpr int kStream = 2;                 // non-temporal
 
 // `bytes` bytes at p + off (none where p is null).
 __device__ __forceinline__ Buffer buffer(const void *p, int64_t off, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(static_cast<const char *>(p)) + off, 0,
                                            p ? static_cast<int>(bytes) : 0, 0x00020000);
 }
+// Stores are ordinary ones: what a step writes is read by the next product.
+// Measured against non-temporal stores: calls of 100 - 250 MB, whose outputs
+// stay in the Infinity Cache, gain 8 - 13 % ([8192, 2560] bf16 forward 36.1 ->
+// 31.3 us), those of 800 MB lose 2 %.
 __device__ __forceinline__ Packed buffer_load(Buffer b, uint32_t at) {
   const native_u4 t = __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0);
   Packed r;
@@ -87,7 +90,7 @@ __device__ __forceinline__ float buffer_load_float(Buffer b, uint32_t at) {
 }
 __device__ __forceinline__ void buffer_store(Buffer b, uint32_t at, const Packed &r) {
   const native_u4 t = {r.v.x, r.v.y, r.v.z, r.v.w};
-  __builtin_amdgcn_raw_buffer_store_b128(t, b, at, 0, kStream);
+  __builtin_amdgcn_raw_buffer_store_b128(t, b, at, 0, 0);
 }
 __device__ __forceinline__ void buffer_store_float(Buffer b, uint32_t at, float v) {
   __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), b, at, 0, 0);
@@ -238,11 +241,16 @@ template <int RPB> __device__ __forceinline__ uint32_t rows_in(int64_t base, int
   return n >= RPB ? RPB : n > 0 ? static_cast<uint32_t>(n) : 0u;
 }
 
+// The second launch bound: waves per SIMD of the blocks a CU has at once.
+constexpr int bwd_bound(int vec, bool layer, bool post, bool pre, bool any, int tpr) {
+  return (bwd_blocks_per_cu(vec, layer, post, pre, any, tpr) * bwd_block(tpr) + 255) / 256;
+}
+
 // Forward.  A block takes runs of rows (chunks) that share a gate row.
 template <typename T, bool LN, bool POST, bool PRE, bool COPY, bool ANY, int TPR>
 __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const StepArgs a) {
   constexpr int V = Tok<T>::VEC;
-  constexpr int BLOCK = fwd_block(TPR), RPB = BLOCK / TPR;
+  constexpr int BLOCK = fwd_block(TPR), RPB = BLOCK / TPR, D = fwd_depth(TPR, ANY);
   __shared__ float lds[RowTotal<TPR, BLOCK, 1>::kFloats];
   int turn = 0;
   const Place<T, TPR, BLOCK, ANY> pl(a);
@@ -259,23 +267,28 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
     const int64_t last = least(first + a.chunk_rows, (group + 1) * a.rows_per_gate);
     load_branch<V, POST>(a, group, pl.c, pl.n, kp);
     if constexpr (POST && LN) load_branch_bias<V>(a, group, pl.c, pl.n, kb);
-    Packed x, r, gf;
-    auto ask = [&](int64_t base) {
+    Packed x[D], r[D], gf[D];
+    auto ask = [&](int u, int64_t base) {
       const int64_t off = base * a.cols * static_cast<int64_t>(sizeof(T));
       const uint32_t bytes = rows_in<RPB>(base, last) * row_bytes;
-      x = pl.load(buffer(a.x, off, bytes));
-      r = pl.load(buffer(a.res, off, bytes));
-      if constexpr (ANY) gf = pl.load(buffer(a.gate_kind == 2 ? a.gate : nullptr, off, bytes));
+      x[u] = pl.load(buffer(a.x, off, bytes));
+      r[u] = pl.load(buffer(a.res, off, bytes));
+      if constexpr (ANY) gf[u] = pl.load(buffer(a.gate_kind == 2 ? a.gate : nullptr, off, bytes));
     };
-    ask(first);
+#pragma unroll
+    for (int u = 0; u < D; ++u) ask(u, first + u * RPB);
 #pragma unroll 1
-    for (int64_t base = first; base < last; base += RPB) {
+    for (int64_t base0 = first; base0 < last; base0 += D * RPB) {
+#pragma unroll
+     for (int u = 0; u < D; ++u) {
+      const int64_t base = base0 + u * RPB;
+      if (u > 0 && base >= last) break;
       const uint32_t rows = rows_in<RPB>(base, last), bytes = rows * row_bytes;
       const int64_t off = base * a.cols * static_cast<int64_t>(sizeof(T));
       float h[V], q[V];
       float m1 = 0.f, v1 = 0.f, m2 = 0.f, v2 = 0.f;
-      Tok<T>::unpack(x, h);
-      Tok<T>::unpack(r, q);
+      Tok<T>::unpack(x[u], h);
+      Tok<T>::unpack(r[u], q);
 #pragma unroll
       for (int j = 0; j < V; ++j) q[j] *= a.res_scale;
       auto copy = [&](const float (&v)[V], void *codes, void *scales) {
@@ -290,14 +303,14 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
       if constexpr (COPY) copy(h, a.x8, a.x8_scale);
       float g[V];
       if constexpr (ANY) {
-        Tok<T>::unpack(gf, g);
+        Tok<T>::unpack(gf[u], g);
 #pragma unroll
         for (int j = 0; j < V; ++j) g[j] = a.gate_kind == 2 ? g[j] : 1.f;
         settle(g);
       }
       settle(h);
       settle(q);
-      ask(base + RPB);
+      ask(u, base + D * RPB);
       auto moments = [&](float &mean, float &var) {
         float s[1] = {0.f};
         if constexpr (LN) {
@@ -324,12 +337,12 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
       }
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float u = (POST && LN ? h[j] - m1 : h[j]) * rho;
+        const float xh = (POST && LN ? h[j] - m1 : h[j]) * rho;
         if constexpr (ANY) {
-          h[j] = fmaf(POST && LN ? fmaf(u, kp[j], kb[j]) : u * kp[j], g[j], q[j]);
+          h[j] = fmaf(POST && LN ? fmaf(xh, kp[j], kb[j]) : xh * kp[j], g[j], q[j]);
         } else {
           if constexpr (POST && LN) q[j] += kb[j];
-          h[j] = fmaf(u, kp[j], q[j]);
+          h[j] = fmaf(xh, kp[j], q[j]);
         }
       }
       const Packed hp = Tok<T>::pack(h);
@@ -356,6 +369,7 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
         if constexpr (LN) buffer_store_float(buffer(a.mean_pre, 4 * base, 4 * rows), stat_out, m2);
         buffer_store_float(buffer(a.var_pre, 4 * base, 4 * rows), stat_out, v2);
       }
+     }
     }
   }
 }
@@ -440,9 +454,10 @@ template <int V, int TPR> struct ColumnSum<V, TPR, true> {
 // Backward.  Each input vector is asked for again, for the next row, right
 // after its last use.
 template <typename T, bool LN, bool POST, bool PRE, bool Q8, bool ANY, int TPR>
-__global__ __launch_bounds__(bwd_block(TPR)) void step_bwd_rows_kernel(const StepArgs a) {
+__global__ __launch_bounds__(bwd_block(TPR), bwd_bound(Tok<T>::VEC, LN, POST, PRE, ANY, TPR))
+void step_bwd_rows_kernel(const StepArgs a) {
   constexpr int V = Tok<T>::VEC;
-  constexpr int BLOCK = bwd_block(TPR), RPB = BLOCK / TPR;
+  constexpr int BLOCK = bwd_block(TPR), RPB = BLOCK / TPR, D = bwd_depth(V, LN, POST, PRE, ANY, TPR);
   constexpr int S = LN ? 2 : 1; // row sums per norm, column sums per norm
   __shared__ float lds[RowTotal<TPR, BLOCK, S>::kFloats];
   __shared__ float fold[RPB > 1 ? BLOCK * V : 1];
@@ -455,20 +470,21 @@ __global__ __launch_bounds__(bwd_block(TPR)) void step_bwd_rows_kernel(const Ste
   constexpr bool TIGHT = TPR == 1024 && V == 8;
   constexpr bool EB_LDS = LN && TIGHT, A_LDS = TIGHT && (ANY || (LN && Q8));
   constexpr bool C_LDS = TIGHT && LN && (ANY || Q8);
-  constexpr bool RELOAD = TIGHT && ANY && LN && POST; // gamma_pre: read per row
   __shared__ float4 eb_lds[EB_LDS ? 2 * TPR * V / 4 : 1], a_lds[A_LDS ? TPR * V / 4 : 1],
       c_lds[C_LDS ? TPR * V / 4 : 1];
   float4 *const e_lds = eb_lds, *const b_lds = eb_lds + (EB_LDS ? TPR * V / 4 : 0);
   ColumnSum<V, TPR, C_LDS> C;
   ColumnSum<V, TPR, EB_LDS> E, B;
   ColumnSum<V, TPR, A_LDS> A;
-  if constexpr (PRE && !RELOAD) load_param<V>(a.gamma_pre, pl.c, pl.n, gn);
+  if constexpr (PRE) load_param<V>(a.gamma_pre, pl.c, pl.n, gn);
   C.clear(c_lds);
   E.clear(e_lds);
 
-  Kept<T, Q8, TPR, BLOCK, ANY> x, h;
-  Packed dh, dy, gf;
-  float m1 = 0.f, v1 = 0.f, m2 = 0.f, v2 = 0.f;
+  struct Row {
+    Kept<T, Q8, TPR, BLOCK, ANY> x, h;
+    Packed dh, dy, gf;
+    float m1, v1, m2, v2;
+  } slot[D];
   // Column sums (times `scale`) of the block's rows-at-a-time to `out`; every
   // thread of the block is here.
   auto flush = [&](float *out, const float (&s)[V], float scale) {
@@ -502,44 +518,51 @@ __global__ __launch_bounds__(bwd_block(TPR)) void step_bwd_rows_kernel(const Ste
     A.clear(a_lds);
     B.clear(b_lds);
     load_branch<V, POST>(a, group, pl.c, pl.n, kp);
-    auto ask_pre = [&](int64_t base) {
+    auto ask_pre = [&](Row &r, int64_t base) {
       const uint32_t rows = rows_in<RPB>(base, last);
       const int64_t off = base * a.cols * static_cast<int64_t>(sizeof(T));
       if constexpr (PRE) {
-        h.ask(a, a.kept_h, a.kept_h_scale, base, rows, pl);
-        dy = pl.load(buffer(a.dy, off, rows * row_bytes));
-        if constexpr (LN) m2 = buffer_load_float(buffer(a.mean_pre, 4 * base, 4 * rows), pl.stat);
-        v2 = buffer_load_float(buffer(a.var_pre, 4 * base, 4 * rows), pl.stat);
+        r.h.ask(a, a.kept_h, a.kept_h_scale, base, rows, pl);
+        r.dy = pl.load(buffer(a.dy, off, rows * row_bytes));
+        if constexpr (LN) r.m2 = buffer_load_float(buffer(a.mean_pre, 4 * base, 4 * rows), pl.stat);
+        r.v2 = buffer_load_float(buffer(a.var_pre, 4 * base, 4 * rows), pl.stat);
       }
-      dh = pl.load(buffer(a.dh, off, rows * row_bytes));
+      r.dh = pl.load(buffer(a.dh, off, rows * row_bytes));
     };
-    auto ask_post = [&](int64_t base) {
+    auto ask_post = [&](Row &r, int64_t base) {
       const uint32_t rows = rows_in<RPB>(base, last);
-      x.ask(a, a.x, a.kept_x_scale, base, rows, pl);
+      r.x.ask(a, a.x, a.kept_x_scale, base, rows, pl);
       if constexpr (ANY)
-        gf = pl.load(buffer(a.gate_kind == 2 ? a.gate : nullptr,
+        r.gf = pl.load(buffer(a.gate_kind == 2 ? a.gate : nullptr,
                             base * a.cols * static_cast<int64_t>(sizeof(T)), rows * row_bytes));
       if constexpr (POST) {
-        if constexpr (LN) m1 = buffer_load_float(buffer(a.mean_post, 4 * base, 4 * rows), pl.stat);
-        v1 = buffer_load_float(buffer(a.var_post, 4 * base, 4 * rows), pl.stat);
+        if constexpr (LN) r.m1 = buffer_load_float(buffer(a.mean_post, 4 * base, 4 * rows), pl.stat);
+        r.v1 = buffer_load_float(buffer(a.var_post, 4 * base, 4 * rows), pl.stat);
       }
     };
-    ask_pre(first);
-    ask_post(first);
+#pragma unroll
+    for (int u = 0; u < D; ++u) {
+      ask_pre(slot[u], first + u * RPB);
+      ask_post(slot[u], first + u * RPB);
+    }
 #pragma unroll 1
-    for (int64_t base = first; base < last; base += RPB) {
+    for (int64_t base0 = first; base0 < last; base0 += D * RPB) {
+#pragma unroll
+     for (int u = 0; u < D; ++u) {
+      const int64_t base = base0 + u * RPB;
+      if (u > 0 && base >= last) break;
+      Row &r = slot[u];
       const uint32_t rows = rows_in<RPB>(base, last);
       const int64_t off = base * a.cols * static_cast<int64_t>(sizeof(T));
       const bool in = RPB == 1 || pl.stat < 4 * rows;
       float t[V];
       if constexpr (PRE) {
-        const float rho = in ? inv_std(v2, a.eps) : 0.f, mu = m2;
+        const float rho = in ? inv_std(r.v2, a.eps) : 0.f, mu = r.m2;
         float s[S], hh[V], d[V];
 #pragma unroll
         for (int i = 0; i < S; ++i) s[i] = 0.f;
-        h.get(a, hh);
-        Tok<T>::unpack(dy, d);
-        if constexpr (RELOAD) load_param<V>(a.gamma_pre, pl.c, pl.n, gn);
+        r.h.get(a, hh);
+        Tok<T>::unpack(r.dy, d);
         C.load(c_lds);
         if constexpr (LN) E.load(e_lds);
 #pragma unroll
@@ -553,25 +576,24 @@ __global__ __launch_bounds__(bwd_block(TPR)) void step_bwd_rows_kernel(const Ste
         }
         C.save(c_lds);
         if constexpr (LN) E.save(e_lds);
-        h.pin();
+        r.h.pin();
         if constexpr (sizeof(T) == 2)
-          asm volatile("" : "+v"(dy.v.x), "+v"(dy.v.y), "+v"(dy.v.z), "+v"(dy.v.w));
+          asm volatile("" : "+v"(r.dy.v.x), "+v"(r.dy.v.y), "+v"(r.dy.v.z), "+v"(r.dy.v.w));
         row_total<TPR, S>(s, lds, turn);
         const float s2 = s[0] * inv, s1 = LN ? s[S - 1] * inv : 0.f;
-        if constexpr (RELOAD) load_param<V>(a.gamma_pre, pl.c, opaque(pl.n), gn);
-        h.get(a, hh);
-        Tok<T>::unpack(dy, d);
-        Tok<T>::unpack(dh, t);
+        r.h.get(a, hh);
+        Tok<T>::unpack(r.dy, d);
+        Tok<T>::unpack(r.dh, t);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           hh[j] = (LN ? hh[j] - mu : hh[j]) * rho;
           t[j] = fmaf(rho, fmaf(d[j], gn[j], -(LN ? fmaf(hh[j], s2, s1) : hh[j] * s2)), t[j]);
         }
       } else {
-        Tok<T>::unpack(dh, t);
+        Tok<T>::unpack(r.dh, t);
       }
       settle(t);
-      ask_pre(base + RPB);
+      ask_pre(r, base + D * RPB);
       {
         float o[V];
 #pragma unroll
@@ -579,11 +601,11 @@ __global__ __launch_bounds__(bwd_block(TPR)) void step_bwd_rows_kernel(const Ste
         pl.put(buffer(a.dres, off, rows * row_bytes),
                buffer(a.accum & NBLAHIP_ACCUM_DRES ? a.dres : nullptr, off, rows * row_bytes), o);
       }
-      const float rho = POST ? in ? inv_std(v1, a.eps) : 0.f : 1.f, mu = POST ? m1 : 0.f;
+      const float rho = POST ? in ? inv_std(r.v1, a.eps) : 0.f : 1.f, mu = POST ? r.m1 : 0.f;
       float m[S], xh[V];
 #pragma unroll
       for (int i = 0; i < S; ++i) m[i] = 0.f;
-      x.get(a, xh);
+      r.x.get(a, xh);
       if constexpr (POST) {
 #pragma unroll
         for (int j = 0; j < V; ++j) xh[j] = (LN ? xh[j] - mu : xh[j]) * rho;
@@ -597,7 +619,7 @@ __global__ __launch_bounds__(bwd_block(TPR)) void step_bwd_rows_kernel(const Ste
           g[j] = t[j] * (POST && LN ? fmaf(xh[j], kp[j], a.branch_scale * g[j]) : xh[j] * kp[j]);
         pl.put(buffer(full ? a.dgate : nullptr, off, rows * row_bytes),
                buffer(full && (a.accum & NBLAHIP_ACCUM_DGATE) ? a.dgate : nullptr, off, rows * row_bytes), g);
-        Tok<T>::unpack(gf, g);
+        Tok<T>::unpack(r.gf, g);
 #pragma unroll
         for (int j = 0; j < V; ++j) t[j] *= full ? g[j] : 1.f;
       }
@@ -619,10 +641,10 @@ __global__ __launch_bounds__(bwd_block(TPR)) void step_bwd_rows_kernel(const Ste
       A.save(a_lds);
       if constexpr (LN && POST) B.save(b_lds);
       if constexpr (POST) {
-        x.pin();
+        r.x.pin();
         row_total<TPR, S>(m, lds, turn);
         const float s2 = m[0] * inv, s1 = LN ? m[S - 1] * inv : 0.f;
-        x.get(a, xh);
+        r.x.get(a, xh);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           xh[j] = (LN ? xh[j] - mu : xh[j]) * rho;
@@ -630,9 +652,10 @@ __global__ __launch_bounds__(bwd_block(TPR)) void step_bwd_rows_kernel(const Ste
         }
       }
       settle(t);
-      ask_post(base + RPB);
+      ask_post(r, base + D * RPB);
       pl.put(buffer(a.dx, off, rows * row_bytes),
              buffer(a.accum & NBLAHIP_ACCUM_DX ? a.dx : nullptr, off, rows * row_bytes), t);
+     }
     }
     if (a.part_post) {
       float *out = a.part_post + chunk * S * a.pitch;
