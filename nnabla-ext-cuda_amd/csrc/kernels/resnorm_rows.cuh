@@ -335,9 +335,10 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
         moments(m1, v1);
         rho = inv_std(v1, a.eps);
       }
+      const float shift1 = -m1 * rho; // 16-bit data: see Kept::unit
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float xh = (POST && LN ? h[j] - m1 : h[j]) * rho;
+        const float xh = !(POST && LN) ? h[j] * rho : V == 8 ? fmaf(h[j], rho, shift1) : (h[j] - m1) * rho;
         if constexpr (ANY) {
           h[j] = fmaf(POST && LN ? fmaf(xh, kp[j], kb[j]) : xh * kp[j], g[j], q[j]);
         } else {
@@ -354,11 +355,12 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
       }
       if constexpr (PRE) {
         moments(m2, v2);
-        const float rho2 = inv_std(v2, a.eps);
+        const float rho2 = inv_std(v2, a.eps), shift2 = -m2 * rho2;
         float y[V];
 #pragma unroll
         for (int j = 0; j < V; ++j)
-          y[j] = LN ? fmaf((h[j] - m2) * rho2, gn[j], bn[j]) : h[j] * rho2 * gn[j];
+          y[j] = !LN ? h[j] * rho2 * gn[j]
+                     : fmaf(V == 8 ? fmaf(h[j], rho2, shift2) : (h[j] - m2) * rho2, gn[j], bn[j]);
         pl.store(buffer(a.y, off, bytes), Tok<T>::pack(y));
       }
       if constexpr (POST) {
@@ -385,6 +387,16 @@ template <typename T, bool Q8, int TPR, int BLOCK, bool ANY> struct Kept {
   __device__ __forceinline__ void get(const StepArgs &, float (&o)[Tok<T>::VEC]) const {
     Tok<T>::unpack(p, o);
   }
+  // (value - mu) * rho.  16-bit data takes one fma, value * rho - mu * rho: off by
+  // 2^-24 |mu| rho, far below what the data resolves; float data is centred first.
+  template <bool CENTRED>
+  __device__ __forceinline__ void unit(const StepArgs &a, float mu, float rho, float (&o)[Tok<T>::VEC]) const {
+    get(a, o);
+    const float shift = -mu * rho;
+#pragma unroll
+    for (int j = 0; j < Tok<T>::VEC; ++j)
+      o[j] = !CENTRED ? o[j] * rho : sizeof(T) == 2 ? fmaf(o[j], rho, shift) : (o[j] - mu) * rho;
+  }
   // Hides the value from the optimiser, so that its widened form is made anew
   // where it is needed instead of being kept in twice the registers.
   __device__ __forceinline__ void pin() {
@@ -402,6 +414,14 @@ template <typename T, int TPR, int BLOCK, bool ANY> struct Kept<T, true, TPR, BL
   }
   __device__ __forceinline__ void get(const StepArgs &a, float (&o)[Tok<T>::VEC]) const {
     act8_decode<Tok<T>::VEC>(q, code, a.format8, o);
+  }
+  // One multiplication takes the scale (a power of two: exact) and rho.
+  template <bool CENTRED>
+  __device__ __forceinline__ void unit(const StepArgs &a, float mu, float rho, float (&o)[Tok<T>::VEC]) const {
+    const float scale = act8_scale(code) * rho, shift = -mu * rho;
+    act8_numbers<Tok<T>::VEC>(q, a.format8, o);
+#pragma unroll
+    for (int j = 0; j < Tok<T>::VEC; ++j) o[j] = CENTRED ? fmaf(o[j], scale, shift) : o[j] * scale;
   }
   __device__ __forceinline__ void pin() { asm volatile("" : "+v"(q.x), "+v"(q.y), "+v"(code)); }
 };
@@ -561,13 +581,12 @@ void step_bwd_rows_kernel(const StepArgs a) {
         float s[S], hh[V], d[V];
 #pragma unroll
         for (int i = 0; i < S; ++i) s[i] = 0.f;
-        r.h.get(a, hh);
+        r.h.template unit<LN>(a, mu, rho, hh);
         Tok<T>::unpack(r.dy, d);
         C.load(c_lds);
         if constexpr (LN) E.load(e_lds);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          hh[j] = (LN ? hh[j] - mu : hh[j]) * rho;
           C.add(c_lds, j, d[j], hh[j]);
           if constexpr (LN) E.add(e_lds, j, d[j], 1.f);
           d[j] *= gn[j];
@@ -581,12 +600,11 @@ void step_bwd_rows_kernel(const StepArgs a) {
           asm volatile("" : "+v"(r.dy.v.x), "+v"(r.dy.v.y), "+v"(r.dy.v.z), "+v"(r.dy.v.w));
         row_total<TPR, S>(s, lds, turn);
         const float s2 = s[0] * inv, s1 = LN ? s[S - 1] * inv : 0.f;
-        r.h.get(a, hh);
+        r.h.template unit<LN>(a, mu, rho, hh);
         Tok<T>::unpack(r.dy, d);
         Tok<T>::unpack(r.dh, t);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          hh[j] = (LN ? hh[j] - mu : hh[j]) * rho;
           t[j] = fmaf(rho, fmaf(d[j], gn[j], -(LN ? fmaf(hh[j], s2, s1) : hh[j] * s2)), t[j]);
         }
       } else {
@@ -605,11 +623,10 @@ void step_bwd_rows_kernel(const StepArgs a) {
       float m[S], xh[V];
 #pragma unroll
       for (int i = 0; i < S; ++i) m[i] = 0.f;
-      r.x.get(a, xh);
-      if constexpr (POST) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) xh[j] = (LN ? xh[j] - mu : xh[j]) * rho;
-      }
+      if constexpr (POST)
+        r.x.template unit<LN>(a, mu, rho, xh);
+      else
+        r.x.get(a, xh);
       if constexpr (ANY) {
         const bool full = a.gate_kind == 2;
         float g[V];
@@ -629,7 +646,7 @@ void step_bwd_rows_kernel(const StepArgs a) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         A.add(a_lds, j, t[j], xh[j]);
-        if constexpr (LN && POST) B.add(b_lds, j, in ? t[j] : 0.f, 1.f);
+        if constexpr (LN && POST) B.add(b_lds, j, t[j], 1.f);
         t[j] *= kp[j];
         if constexpr (POST) {
           if constexpr (LN) m[S - 1] += t[j];
@@ -641,15 +658,13 @@ void step_bwd_rows_kernel(const StepArgs a) {
       A.save(a_lds);
       if constexpr (LN && POST) B.save(b_lds);
       if constexpr (POST) {
-        r.x.pin();
+        if constexpr (PRE) r.x.pin(); // (the first norm alone has registers to keep xh)
         row_total<TPR, S>(m, lds, turn);
         const float s2 = m[0] * inv, s1 = LN ? m[S - 1] * inv : 0.f;
-        r.x.get(a, xh);
+        if constexpr (PRE) r.x.template unit<LN>(a, mu, rho, xh);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          xh[j] = (LN ? xh[j] - mu : xh[j]) * rho;
+        for (int j = 0; j < V; ++j)
           t[j] = rho * (t[j] - (LN ? fmaf(xh[j], s2, s1) : xh[j] * s2));
-        }
       }
       settle(t);
       ask_post(r, base + D * RPB);

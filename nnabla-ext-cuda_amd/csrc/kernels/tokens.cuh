@@ -249,27 +249,29 @@ __device__ __forceinline__ float act8_scale(uint32_t code) {
   return code == 255u ? __builtin_nanf("") : __builtin_bit_cast(float, code << 23);
 }
 
+// The numbers that the codes are, without their scale.
 template <int VEC>
-__device__ __forceinline__ void act8_decode(uint2 q, uint32_t code, int format, float (&o)[VEC]) {
-  const float s = act8_scale(code);
+__device__ __forceinline__ void act8_numbers(uint2 q, int format, float (&o)[VEC]) {
   const uint32_t w[2] = {q.x, q.y};
   if (format == kAct8Int8) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      // biased to unsigned: the byte-to-float conversion is one instruction.
-      // (The bias goes off before the scale is multiplied in: 128 times the
-      // largest scales is past the largest float.)
-      const uint32_t u = ((w[j / 4] ^ 0x80808080u) >> (8 * (j & 3))) & 0xffu;
-      o[j] = (static_cast<float>(u) - 128.f) * s;
-    }
+    for (int j = 0; j < VEC; ++j) // (one instruction: conversion of a sign-extended byte)
+      o[j] = static_cast<float>(static_cast<int>(static_cast<int8_t>(w[j / 4] >> (8 * (j & 3)))));
   } else {
 #pragma unroll
     for (int j = 0; j < VEC; j += 4) {
       const native_f2 a = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[j / 4]), false);
       const native_f2 b = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[j / 4]), true);
-      o[j] = a.x * s; o[j + 1] = a.y * s; o[j + 2] = b.x * s; o[j + 3] = b.y * s;
+      o[j] = a.x; o[j + 1] = a.y; o[j + 2] = b.x; o[j + 3] = b.y;
     }
   }
+}
+template <int VEC>
+__device__ __forceinline__ void act8_decode(uint2 q, uint32_t code, int format, float (&o)[VEC]) {
+  const float s = act8_scale(code);
+  act8_numbers<VEC>(q, format, o);
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) o[j] *= s;
 }
 
 // n of VEC codes at p, zeros behind them.
