@@ -109,6 +109,17 @@ NNABLA_HIP_EXPORT nnabla_hip_function *nnabla_hip_create_tensor_normalization(
 NNABLA_HIP_EXPORT nnabla_hip_function *nnabla_hip_create_weight_standardization(
     const char *backends, const char *array_class, const char *device_id, int channel_axis,
     float eps);
+/* Functions of transformer blocks (no counterpart in the reference; inputs and
+ * outputs: host/include/nbla/hip/function/rms_normalization.hpp and
+ * residual_normalization.hpp).  batch_axis: the leading axes.  checkpoint: "",
+ * "int8" or "e4m3".  norm: "rms" or "layer". */
+NNABLA_HIP_EXPORT nnabla_hip_function *nnabla_hip_create_rms_normalization(
+    const char *backends, const char *array_class, const char *device_id, const int *batch_axis,
+    int n_batch_axis, float eps, int no_scale, const char *checkpoint);
+NNABLA_HIP_EXPORT nnabla_hip_function *nnabla_hip_create_residual_normalization(
+    const char *backends, const char *array_class, const char *device_id, const int *batch_axis,
+    int n_batch_axis, const char *norm, int post, int pre, int residual, int gate, float res_scale,
+    float branch_scale, float eps, int no_scale, int no_bias, const char *checkpoint);
 NNABLA_HIP_EXPORT void nnabla_hip_function_delete(nnabla_hip_function *f);
 NNABLA_HIP_EXPORT const char *nnabla_hip_function_name(nnabla_hip_function *f);
 

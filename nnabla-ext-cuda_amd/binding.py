@@ -49,6 +49,9 @@ SIGNATURES = {
     "nnabla_hip_create_instance_normalization": (_P, [_S, _S, _S, _I, _IP, _I, _F, _I, _I]),
     "nnabla_hip_create_tensor_normalization": (_P, [_S, _S, _S, _IP, _I, _F, _I, _I]),
     "nnabla_hip_create_weight_standardization": (_P, [_S, _S, _S, _I, _F]),
+    "nnabla_hip_create_rms_normalization": (_P, [_S, _S, _S, _IP, _I, _F, _I, _S]),
+    "nnabla_hip_create_residual_normalization": (_P, [_S, _S, _S, _IP, _I, _S] + [_I] * 4 + [_F] * 3 +
+                                                 [_I, _I, _S]),
     "nnabla_hip_function_delete": (None, [_P]),
     "nnabla_hip_function_name": (_S, [_P]),
     "nnabla_hip_function_setup": (_I, [_P, _PP, _I, _PP, _I]),
@@ -352,3 +355,23 @@ def TensorNormalization(ctx, axes=(1,), eps=1e-5, no_scale=False, no_bias=False)
 def WeightStandardization(ctx, channel_axis=0, eps=1e-5):
     return Function(lib().nnabla_hip_create_weight_standardization(
         *_ctx_args(ctx), channel_axis, eps))
+
+
+def RMSNormalization(ctx, batch_axis=(0,), eps=1e-5, no_scale=False, checkpoint=""):
+    """Inputs x[, gamma]; output y.  checkpoint "int8" / "e4m3": the backward reads
+    an 8-bit copy of x that the forward keeps."""
+    ba, n = _ints(list(batch_axis))
+    return Function(lib().nnabla_hip_create_rms_normalization(
+        *_ctx_args(ctx), ba, n, eps, int(no_scale), checkpoint.encode()))
+
+
+def ResidualNormalization(ctx, batch_axis=(0,), norm="rms", post=True, pre=True, residual=True,
+                          gate=False, res_scale=1.0, branch_scale=1.0, eps=1e-5, no_scale=False,
+                          no_bias=False, checkpoint=""):
+    """h = res_scale*res + branch_scale*gate*post(x), y = pre(h).  Inputs, those
+    that are there: x, res, gate, beta_post, gamma_post, beta_pre, gamma_pre (betas
+    with norm "layer"); outputs h[, y]."""
+    ba, n = _ints(list(batch_axis))
+    return Function(lib().nnabla_hip_create_residual_normalization(
+        *_ctx_args(ctx), ba, n, norm.encode(), int(post), int(pre), int(residual), int(gate), res_scale,
+        branch_scale, eps, int(no_scale), int(no_bias), checkpoint.encode()))

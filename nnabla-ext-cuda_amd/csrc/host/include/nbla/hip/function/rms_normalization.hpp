@@ -1,0 +1,54 @@
+// RMSNormalization: y = x / sqrt(mean(x^2) + eps) * gamma over the axes that are
+// not batch axes.  No counterpart in the reference; the class follows
+// LayerNormalizationHip<T> (arguments, statistics kept for backward, parameters
+// that may be stored in half).
+//
+// Inputs [x] (no_scale) or [x, gamma]; output [y].  checkpoint "int8" / "e4m3":
+// the forward keeps an 8-bit copy of x, and the backward reads that instead of
+// the input's data.
+#pragma once
+
+#include <nbla/function_registry.hpp>
+#include <nbla/hip/common.hpp>
+#include <nbla/hip/hip.hpp>
+#include <nbla/hip/utils/act8_copy.hpp>
+#include <nbla/hip/utils/param_stage.hpp>
+
+namespace nbla {
+
+NBLA_REGISTER_FUNCTION_HEADER(RMSNormalization, const vector<int> &, float, bool, const string &);
+
+template <typename T> class RMSNormalizationHip : public Function {
+protected:
+  int device_;
+  vector<int> batch_axis_;
+  float eps_;
+  bool no_scale_;
+  int format8_;
+  Size_t rows_ = 0, cols_ = 0;
+  Variable ms_; // float32 mean squares kept for backward
+  Act8Copy x8_;
+  Variable workspace_;
+  size_t workspace_bytes_ = 0;
+  Variable stage_; // float32 staging of parameters stored in half (ParamStage)
+
+public:
+  RMSNormalizationHip(const Context &ctx, const vector<int> &batch_axis, float eps, bool no_scale,
+                      const string &checkpoint)
+      : Function(ctx), device_(std::stoi(ctx.device_id)), batch_axis_(batch_axis), eps_(eps),
+        no_scale_(no_scale), format8_(act8_format(checkpoint)) {}
+  virtual ~RMSNormalizationHip() {}
+  virtual string name() { return "RMSNormalizationHip"; }
+  virtual int min_inputs() { return 1; }
+  virtual int min_outputs() { return 1; }
+  virtual vector<string> allowed_array_classes() {
+    return SingletonManager::get<Hip>()->array_classes();
+  }
+
+protected:
+  virtual void setup_impl(const Variables &inputs, const Variables &outputs);
+  virtual void forward_impl(const Variables &inputs, const Variables &outputs);
+  virtual void backward_impl(const Variables &inputs, const Variables &outputs,
+                             const vector<bool> &propagate_down, const vector<bool> &accum);
+};
+} // namespace nbla

@@ -10,6 +10,8 @@
 #include <nbla/function/layer_normalization.hpp>
 #include <nbla/function/tensor_normalization.hpp>
 #include <nbla/function/weight_standardization.hpp>
+#include <nbla/hip/function/residual_normalization.hpp>
+#include <nbla/hip/function/rms_normalization.hpp>
 #include <nbla/hip/hip.hpp>
 #include <nbla/hip/init.hpp>
 #include <nbla/variable.hpp>
@@ -368,6 +370,36 @@ nnabla_hip_function *nnabla_hip_create_weight_standardization(const char *backen
   guarded([&] {
     out = wrap(create_WeightStandardization(make_ctx(backends, array_class, device_id),
                                             channel_axis, eps));
+  });
+  return out;
+}
+
+nnabla_hip_function *nnabla_hip_create_rms_normalization(const char *backends,
+                                                         const char *array_class,
+                                                         const char *device_id,
+                                                         const int *batch_axis, int n_batch_axis,
+                                                         float eps, int no_scale,
+                                                         const char *checkpoint) {
+  nnabla_hip_function *out = nullptr;
+  guarded([&] {
+    const vector<int> ba(batch_axis, batch_axis + n_batch_axis);
+    out = wrap(create_RMSNormalization(make_ctx(backends, array_class, device_id), ba, eps,
+                                       no_scale != 0, string(checkpoint ? checkpoint : "")));
+  });
+  return out;
+}
+
+nnabla_hip_function *nnabla_hip_create_residual_normalization(
+    const char *backends, const char *array_class, const char *device_id, const int *batch_axis,
+    int n_batch_axis, const char *norm, int post, int pre, int residual, int gate, float res_scale,
+    float branch_scale, float eps, int no_scale, int no_bias, const char *checkpoint) {
+  nnabla_hip_function *out = nullptr;
+  guarded([&] {
+    const vector<int> ba(batch_axis, batch_axis + n_batch_axis);
+    out = wrap(create_ResidualNormalization(
+        make_ctx(backends, array_class, device_id), ba, string(norm ? norm : ""), post != 0, pre != 0,
+        residual != 0, gate != 0, res_scale, branch_scale, eps, no_scale != 0, no_bias != 0,
+        string(checkpoint ? checkpoint : "")));
   });
   return out;
 }

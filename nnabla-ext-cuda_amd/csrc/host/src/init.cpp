@@ -1,5 +1,5 @@
 // init_hip(): registration of the "hip" backend (src/nbla/cuda/init.cpp.tmpl:65-270
-// is the reference's equivalent; here the table is five functions by two type
+// is the reference's equivalent; here the table is nine functions by two type
 // configs, written out by hand instead of generated from yaml).
 #include <mutex>
 
@@ -11,6 +11,8 @@
 #include <nbla/hip/function/group_normalization.hpp>
 #include <nbla/hip/function/instance_normalization.hpp>
 #include <nbla/hip/function/layer_normalization.hpp>
+#include <nbla/hip/function/residual_normalization.hpp>
+#include <nbla/hip/function/rms_normalization.hpp>
 #include <nbla/hip/function/tensor_normalization.hpp>
 #include <nbla/hip/function/weight_standardization.hpp>
 #include <nbla/hip/hip.hpp>
@@ -29,6 +31,10 @@ NBLA_REGISTER_FUNCTION_SOURCE(InstanceNormalization, int, const vector<int> &, f
 NBLA_REGISTER_FUNCTION_SOURCE(TensorNormalization, const vector<int> &, float, bool, bool);
 NBLA_REGISTER_FUNCTION_SOURCE(WeightStandardization, int, float);
 #endif
+// Functions of this backend alone: no core owns their registries.
+NBLA_REGISTER_FUNCTION_SOURCE(RMSNormalization, const vector<int> &, float, bool, const string &);
+NBLA_REGISTER_FUNCTION_SOURCE(ResidualNormalization, const vector<int> &, const string &, bool, bool,
+                              bool, bool, float, float, float, bool, bool, const string &);
 
 void init_hip() {
   static std::mutex mtx;
@@ -120,6 +126,21 @@ void init_hip() {
                               int, float);
   NBLA_REGISTER_FUNCTION_IMPL(WeightStandardization, WeightStandardizationHip_half, "hip:half", int,
                               float);
+
+  typedef RMSNormalizationHip<float> RMSNormalizationHip_float;
+  typedef RMSNormalizationHip<Half> RMSNormalizationHip_half;
+  NBLA_REGISTER_FUNCTION_IMPL(RMSNormalization, RMSNormalizationHip_float, "hip:float",
+                              const vector<int> &, float, bool, const string &);
+  NBLA_REGISTER_FUNCTION_IMPL(RMSNormalization, RMSNormalizationHip_half, "hip:half",
+                              const vector<int> &, float, bool, const string &);
+  typedef ResidualNormalizationHip<float> ResidualNormalizationHip_float;
+  typedef ResidualNormalizationHip<Half> ResidualNormalizationHip_half;
+  NBLA_REGISTER_FUNCTION_IMPL(ResidualNormalization, ResidualNormalizationHip_float, "hip:float",
+                              const vector<int> &, const string &, bool, bool, bool, bool, float, float,
+                              float, bool, bool, const string &);
+  NBLA_REGISTER_FUNCTION_IMPL(ResidualNormalization, ResidualNormalizationHip_half, "hip:half",
+                              const vector<int> &, const string &, bool, bool, bool, bool, float, float,
+                              float, bool, bool, const string &);
 
   is_initialized = true;
 }
