@@ -45,12 +45,15 @@ struct StepArgs {
   float res_scale = 1.f, branch_scale = 1.f, eps = 0.f;
 };
 
+// Forms of the row kernels (resnorm_rows.cuh).
+enum StepMode { kWhole = 0, kRagged = 1, kAny = 2 };
+
 // What selects a kernel.
 struct StepPlan {
   int dtype = 0;
   bool layer = false, post = false, pre = false;
   bool kept8 = false;            // backward: x and h are 8-bit copies
-  bool any = false;              // the form of the row kernels for every call (resnorm_rows.cuh)
+  int mode = 0;                  // StepMode
   int tpr = 0;                   // threads per row; 0: the kernels for long rows
 };
 
@@ -69,25 +72,27 @@ constexpr int bwd_block(int tpr) { return tpr == 192 ? 384 : tpr < 512 && tpr !=
 // compiler needs without a limit: 56 - 119 registers a thread, 76 - 148 with
 // `any`), and from them how many blocks a CU has at once: as many as are
 // launched, each walking its share of the rows.
-constexpr int bwd_waves(int vec, bool layer, bool post, bool pre, bool any, int tpr) {
+constexpr int bwd_waves(int vec, bool layer, bool post, bool pre, bool q8, int mode, int tpr) {
+  const bool both = post && pre;
   if (tpr == 1024) return 4;
-  if (vec == 4) return any && layer && post && pre ? 4 : any || (layer && post && pre) ? 5 : 6;
-  if (layer) return (post && pre ? 4 : pre ? 4 : 5) - (any ? 1 : 0);
-  return (pre ? 5 : 6) - (any ? (pre ? 1 : 2) : 0);
+  if (vec == 4) return mode == kAny && layer && both ? 4 : mode != kWhole || (layer && both) ? 5 : 6;
+  if (layer) return (pre ? 4 : 5) - (mode != kWhole ? 1 : 0);
+  return mode == kWhole ? (pre ? 5 : 6) : mode == kRagged && !(both && q8) ? 5 : 4;
 }
-constexpr int bwd_blocks_per_cu(int vec, bool layer, bool post, bool pre, bool any, int tpr) {
-  const int n = 256 * bwd_waves(vec, layer, post, pre, any, tpr) / bwd_block(tpr);
+constexpr int bwd_blocks_per_cu(int vec, bool layer, bool post, bool pre, bool q8, int mode, int tpr) {
+  const int n = 256 * bwd_waves(vec, layer, post, pre, q8, mode, tpr) / bwd_block(tpr);
   return n > 0 ? n : 1;
 }
 // Rows whose loads are in flight ahead of the one in hand: two where a CU has one
 // block, which otherwise stands still while its next row arrives ([8192, 8192]
-// bf16 175 -> 158 us; more blocks per CU do not gain), unless the registers of
-// a block of 1024 are full.
-constexpr int bwd_depth(int vec, bool layer, bool post, bool pre, bool any, int tpr) {
-  const bool full = tpr == 1024 && (vec == 8 ? any || (layer && post && pre) : any && layer);
-  return bwd_blocks_per_cu(vec, layer, post, pre, any, tpr) == 1 && !full ? 2 : 1;
+// bf16 175 -> 158 us), unless the registers of a block of 1024 are full; and in
+// the RMS step at two blocks ([8192, 4096] bf16 162 -> 159).
+constexpr int bwd_depth(int vec, bool layer, bool post, bool pre, bool q8, int mode, int tpr) {
+  const bool full = tpr == 1024 && (vec == 8 ? mode != kWhole || (layer && post && pre) : mode != kWhole && layer);
+  const int blocks = bwd_blocks_per_cu(vec, layer, post, pre, q8, mode, tpr);
+  return (blocks == 1 && !full) || (blocks == 2 && vec == 8 && !layer && mode == kWhole && tpr == 512) ? 2 : 1;
 }
-constexpr int fwd_depth(int tpr, bool any) { return tpr >= 256 && !(any && tpr == 1024) ? 2 : 1; }
+constexpr int fwd_depth(int tpr, int mode) { return tpr >= 256 && !(mode != kWhole && tpr == 1024) ? 2 : 1; }
 
 int launch_step_fwd_f32(const StepPlan &pl, const StepArgs &a, hipStream_t st);
 int launch_step_fwd_f16(const StepPlan &pl, const StepArgs &a, hipStream_t st);

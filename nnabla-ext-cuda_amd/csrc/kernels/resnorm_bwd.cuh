@@ -8,17 +8,17 @@
 
 namespace nblahip {
 
-template <typename T, bool LN, bool POST, bool PRE, bool Q8, bool ANY>
+template <typename T, bool LN, bool POST, bool PRE, bool Q8, int MODE>
 bool launch_bwd_rows(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
-  // the one form that does not fit the registers of a block of 1024
+  // the form that does not fit the registers of a block of 1024
   // (step_bwd_is_long keeps it away)
-  constexpr int MOST = LN && POST && PRE && ANY && sizeof(T) == 2 ? 768 : 1024;
+  constexpr int MOST = LN && POST && PRE && MODE != kWhole && sizeof(T) == 2 ? 768 : 1024;
   switch (pl.tpr) {
 #define NBLAHIP_CASE(TPR)                                                                         \
   case TPR:                                                                                       \
     if constexpr (TPR <= MOST) {                                                                  \
       NBLAHIP_LAUNCH("step_bwd_rows_kernel",                                                      \
-                     (step_bwd_rows_kernel<T, LN, POST, PRE, Q8, ANY, TPR>),                      \
+                     (step_bwd_rows_kernel<T, LN, POST, PRE, Q8, MODE, TPR>),                      \
                      dim3(static_cast<unsigned>(a.grid)), dim3(bwd_block(TPR)), 0, st, a);      \
       return true;                                                                                \
     } else {                                                                                      \
@@ -33,8 +33,9 @@ bool launch_bwd_rows(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
 template <typename T, bool LN, bool POST, bool PRE, bool Q8>
 int launch_bwd_kind(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
   if (pl.tpr != 0) {
-    const bool known = pl.any ? launch_bwd_rows<T, LN, POST, PRE, Q8, true>(pl, a, st)
-                              : launch_bwd_rows<T, LN, POST, PRE, Q8, false>(pl, a, st);
+    const bool known = pl.mode == kWhole    ? launch_bwd_rows<T, LN, POST, PRE, Q8, kWhole>(pl, a, st)
+                       : pl.mode == kRagged ? launch_bwd_rows<T, LN, POST, PRE, Q8, kRagged>(pl, a, st)
+                                            : launch_bwd_rows<T, LN, POST, PRE, Q8, kAny>(pl, a, st);
     return known ? last_launch_status() : NBLAHIP_EINVAL; // (the workspace is not the long rows')
   }
   const dim3 rows(static_cast<unsigned>(std::min<int64_t>(a.rows, 1 << 20)));

@@ -7,13 +7,13 @@
 
 namespace nblahip {
 
-template <typename T, bool LN, bool POST, bool PRE, bool COPY, bool ANY>
+template <typename T, bool LN, bool POST, bool PRE, bool COPY, int MODE>
 bool launch_fwd_rows(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
   switch (pl.tpr) {
 #define NBLAHIP_CASE(TPR)                                                                         \
   case TPR:                                                                                       \
     NBLAHIP_LAUNCH("step_fwd_rows_kernel",                                                        \
-                   (step_fwd_rows_kernel<T, LN, POST, PRE, COPY, ANY, TPR>),                      \
+                   (step_fwd_rows_kernel<T, LN, POST, PRE, COPY, MODE, TPR>),                      \
                    dim3(static_cast<unsigned>(a.grid)), dim3(fwd_block(TPR)), 0, st, a);        \
     return true;
     NBLAHIP_STEP_LAYOUTS(NBLAHIP_CASE)
@@ -27,10 +27,11 @@ int launch_fwd_kind(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
   const bool copy = a.x8 || a.h8;
   if (pl.tpr != 0) {
     const bool known =
-        pl.any ? copy ? launch_fwd_rows<T, LN, POST, PRE, true, true>(pl, a, st)
-                      : launch_fwd_rows<T, LN, POST, PRE, false, true>(pl, a, st)
-               : copy ? launch_fwd_rows<T, LN, POST, PRE, true, false>(pl, a, st)
-                      : launch_fwd_rows<T, LN, POST, PRE, false, false>(pl, a, st);
+        pl.mode == kWhole ? copy ? launch_fwd_rows<T, LN, POST, PRE, true, kWhole>(pl, a, st)
+                                 : launch_fwd_rows<T, LN, POST, PRE, false, kWhole>(pl, a, st)
+        : copy                   ? launch_fwd_rows<T, LN, POST, PRE, true, kAny>(pl, a, st)
+        : pl.mode == kRagged     ? launch_fwd_rows<T, LN, POST, PRE, false, kRagged>(pl, a, st)
+                                 : launch_fwd_rows<T, LN, POST, PRE, false, kAny>(pl, a, st);
     return known ? last_launch_status() : NBLAHIP_EINVAL;
   }
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(a.rows, 1 << 20)));

@@ -107,7 +107,7 @@ int64_t shared_gate_rows(const StepArgs &a, int64_t gate_rows) {
 
 // The backward's only form whose rows of 1024 threads do not fit the registers.
 bool step_bwd_is_long(const StepPlan &pl) {
-  return pl.tpr == 1024 && pl.dtype != NBLAHIP_F32 && pl.layer && pl.post && pl.pre && pl.any;
+  return pl.tpr == 1024 && pl.dtype != NBLAHIP_F32 && pl.layer && pl.post && pl.pre && pl.mode != kWhole;
 }
 
 // The backward's split, and its workspace laid out from `ws` (null: sizes only).
@@ -120,7 +120,7 @@ size_t plan_bwd(StepArgs &a, StepPlan &pl, int64_t gate_rows, char *ws) {
     a.grid = static_cast<int>(std::min<int64_t>(a.chunks, 1 << 30));
   } else {
     const int block = bwd_block(pl.tpr);
-    const int64_t blocks = kCus * bwd_blocks_per_cu(vec_of(pl.dtype), pl.layer, pl.post, pl.pre, pl.any, pl.tpr);
+    const int64_t blocks = kCus * bwd_blocks_per_cu(vec_of(pl.dtype), pl.layer, pl.post, pl.pre, pl.kept8, pl.mode, pl.tpr);
     plan_chunks(a, gate_rows, blocks, block / pl.tpr);
     a.grid = static_cast<int>(std::min<int64_t>(a.chunks, blocks));
   }
@@ -307,8 +307,9 @@ int step_fwd(StepArgs a, StepPlan pl, int64_t gate_rows, hipStream_t st) {
   al.write(a.h8_scale, qs);
   if (al.bad()) return NBLAHIP_EALIAS;
   pick_layout(pl, a.cols);
-  pl.any = a.gate_kind == NBLAHIP_GATE_FULL ||
-           !whole_vectors(pl.dtype, a.cols, {a.x, a.res, a.h, a.y}, {a.x8, a.h8});
+  pl.mode = a.gate_kind == NBLAHIP_GATE_FULL                                               ? kAny
+            : whole_vectors(pl.dtype, a.cols, {a.x, a.res, a.h, a.y}, {a.x8, a.h8}) ? kWhole
+                                                                                    : kRagged;
   gate_rows = shared_gate_rows(a, gate_rows);
   const int block = pl.tpr ? fwd_block(pl.tpr) : 1024;
   const int64_t blocks = kCus * (2048 / block);
@@ -331,10 +332,11 @@ int step_bwd(StepArgs a, StepPlan pl, int64_t gate_rows, void *ws, size_t ws_byt
   if (pl.kept8 && !format_ok(a.format8)) return NBLAHIP_EINVAL;
   gate_rows = shared_gate_rows(a, gate_rows);
   const bool full = a.gate_kind == NBLAHIP_GATE_FULL;
-  pl.any = full || (a.dx && (a.accum & NBLAHIP_ACCUM_DX)) || (a.dres && (a.accum & NBLAHIP_ACCUM_DRES)) ||
-           !whole_vectors(pl.dtype, a.cols, {a.dh, a.dy, a.dx, a.dres}, {}) ||
-           !(pl.kept8 ? whole_vectors(pl.dtype, a.cols, {}, {a.x, a.kept_h})
-                      : whole_vectors(pl.dtype, a.cols, {a.x, a.kept_h}, {}));
+  const bool adds = (a.dx && (a.accum & NBLAHIP_ACCUM_DX)) || (a.dres && (a.accum & NBLAHIP_ACCUM_DRES));
+  const bool whole = whole_vectors(pl.dtype, a.cols, {a.dh, a.dy, a.dx, a.dres}, {}) &&
+                     (pl.kept8 ? whole_vectors(pl.dtype, a.cols, {}, {a.x, a.kept_h})
+                               : whole_vectors(pl.dtype, a.cols, {a.x, a.kept_h}, {}));
+  pl.mode = full || adds ? kAny : whole ? kWhole : kRagged;
   const size_t need = plan_bwd(a, pl, gate_rows, static_cast<char *>(ws));
   if (need && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0 || ws_bytes < need))
     return NBLAHIP_EWORKSPACE;
@@ -523,11 +525,14 @@ size_t nblahip_resnorm_bwd_workspace_bytes(int64_t rows, int64_t cols, int gate_
   a.gate_kind = gate_kind;
   const int64_t g = shared_gate_rows(a, gate_rows);
   size_t most = 0; // over the forms a call of these sizes may take
-  for (const bool any : {false, true}) {
-    StepArgs b = a;
-    StepPlan q = pl;
-    q.any = any;
-    most = std::max(most, plan_bwd(b, q, g, nullptr));
+  for (const int mode : {kWhole, kRagged, kAny}) {
+    for (const bool kept8 : {false, true}) {
+      StepArgs b = a;
+      StepPlan q = pl;
+      q.mode = mode;
+      q.kept8 = kept8;
+      most = std::max(most, plan_bwd(b, q, g, nullptr));
+    }
   }
   return most;
 }

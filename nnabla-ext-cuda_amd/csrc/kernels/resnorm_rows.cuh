@@ -17,11 +17,15 @@
 // absent tensor, a row past the end and a thread past the columns have no
 // records in range: loads give 0, stores are dropped.
 //
-// ANY = false: rows of whole vectors, 16-byte aligned, no gate per element, no
-// accumulation onto dx / dres: the calls models make.  ANY = true: everything
-// else of these widths.  A row that ends inside a vector is read as the vector
-// that ends where the row ends, shifted down, and written in pieces of 8, 4 and
-// 2 bytes; nothing outside the row is touched.
+// Three forms (StepMode):
+//   kWhole : rows of whole vectors, 16-byte aligned, no gate per element, no
+//            accumulation onto dx / dres: the calls models make;
+//   kRagged: rows or tensors at any element.  A row that ends inside a vector is
+//            read as the vector that ends where the row ends, shifted down, and
+//            written in pieces of 8, 4 and 2 bytes; nothing outside the row is
+//            touched;
+//   kAny   : that, a gate per element and accumulation (absent ones cost loads
+//            and stores that the bounds check drops).
 #pragma once
 
 #include "resnorm_long.cuh"
@@ -69,16 +73,18 @@ __device__ __forceinline__ void row_total(float (&v)[N], float (&lds)[CAP], int 
 
 typedef __amdgpu_buffer_rsrc_t Buffer;
 constexpr uint32_t kOutside = 0x7fffffffu; // an offset past every buffer here
+constexpr int kStream = 2;                 // non-temporal
 
 // `bytes` bytes at p + off (none where p is null).
 __device__ __forceinline__ Buffer buffer(const void *p, int64_t off, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(static_cast<const char *>(p)) + off, 0,
                                            p ? static_cast<int>(bytes) : 0, 0x00020000);
 }
-// Stores are ordinary ones: what a step writes is read by the next product.
-// Measured against non-temporal stores: calls of 100 - 250 MB, whose outputs
-// stay in the Infinity Cache, gain 8 - 13 % ([8192, 2560] bf16 forward 36.1 ->
-// 31.3 us), those of 800 MB lose 2 %.
+// Tensors are stored non-temporally: 134 - 202 MB calls gain 3 - 20 % over ordinary
+// stores ([8192, 2560] bf16 pre-norm forward 35.7 -> 28.5 us, [4096, 8192] RMS
+// backward 43.4 -> 41.5), the largest up to 4 %; one loses 2 % ([16384, 4096]
+// forward).  (Measured with outputs that are not written twice: a loop that
+// writes the same buffers again finds them in the cache and shows the opposite.)
 __device__ __forceinline__ Packed buffer_load(Buffer b, uint32_t at) {
   const native_u4 t = __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0);
   Packed r;
@@ -90,7 +96,7 @@ __device__ __forceinline__ float buffer_load_float(Buffer b, uint32_t at) {
 }
 __device__ __forceinline__ void buffer_store(Buffer b, uint32_t at, const Packed &r) {
   const native_u4 t = {r.v.x, r.v.y, r.v.z, r.v.w};
-  __builtin_amdgcn_raw_buffer_store_b128(t, b, at, 0, 0);
+  __builtin_amdgcn_raw_buffer_store_b128(t, b, at, 0, kStream);
 }
 __device__ __forceinline__ void buffer_store_float(Buffer b, uint32_t at, float v) {
   __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), b, at, 0, 0);
@@ -118,20 +124,21 @@ template <int N> __device__ __forceinline__ void settle(float (&v)[N]) {
 
 // Where a thread's vector lies in the rows a block has in hand, in bytes from
 // the first of them: of a tensor of the storage type, of 8-bit codes, of their
-// scales, of a row statistic.  With ANY the thread a row ends in reads the
+// scales, of a row statistic.  Of ragged rows the thread a row ends in reads the
 // vector `drop` elements further ahead, and writes the first `n` of its own.
-template <typename T, int TPR, int BLOCK, bool ANY> struct Place {
+template <typename T, int TPR, int BLOCK, int MODE> struct Place {
   static constexpr int V = Tok<T>::VEC;
   static constexpr uint32_t SZ = sizeof(T);
+  static constexpr bool RAGGED = MODE != kWhole;
   uint32_t wide, codes, scale, stat;
-  uint32_t drop; // ANY only
+  uint32_t drop; // ragged rows only
   int c, n;      // the thread's first column, and how many it has
   __device__ __forceinline__ Place(const StepArgs &a) {
     const uint32_t cols = static_cast<uint32_t>(a.cols);
     const uint32_t sub = BLOCK == TPR ? 0 : threadIdx.x / TPR;
     c = (threadIdx.x % TPR) * V;
     n = columns_left(a.cols - c, V);
-    drop = ANY && n > 0 ? V - n : 0;
+    drop = RAGGED && n > 0 ? V - n : 0;
     wide = n > 0 ? (sub * cols + c - drop) * SZ : kOutside;
     codes = n > 0 ? sub * cols + c - drop : kOutside;
     scale = n > 0 ? sub * static_cast<uint32_t>(a.groups8) + c / kAct8Group : kOutside;
@@ -139,7 +146,7 @@ template <typename T, int TPR, int BLOCK, bool ANY> struct Place {
   }
   __device__ __forceinline__ Packed load(Buffer b) const {
     Packed r = buffer_load(b, wide);
-    if constexpr (ANY) r.v = shift_down_bits(r.v, drop * 8u * SZ);
+    if constexpr (RAGGED) r.v = shift_down_bits(r.v, drop * 8u * SZ);
     return r;
   }
   // Offsets of the pieces a vector that is cut short is written in.
@@ -147,7 +154,7 @@ template <typename T, int TPR, int BLOCK, bool ANY> struct Place {
     return n > 0 ? at + drop * size : kOutside;
   }
   __device__ __forceinline__ void store(Buffer b, const Packed &r) const {
-    if constexpr (!ANY) {
+    if constexpr (!RAGGED) {
       buffer_store(b, wide, r);
     } else {
       buffer_store(b, n == V ? wide : kOutside, r);
@@ -167,7 +174,7 @@ template <typename T, int TPR, int BLOCK, bool ANY> struct Place {
   }
   // onto what `old` (a buffer without records: nothing) holds there
   __device__ __forceinline__ void put(Buffer b, Buffer old, const float (&o)[V]) const {
-    if constexpr (ANY) {
+    if constexpr (MODE == kAny) {
       float sum[V];
       Tok<T>::unpack(load(old), sum);
 #pragma unroll
@@ -185,21 +192,21 @@ template <typename T, int TPR, int BLOCK, bool ANY> struct Place {
     } else {
       q.x = __builtin_amdgcn_raw_buffer_load_b32(b, codes, 0, 0);
     }
-    if constexpr (ANY) {
+    if constexpr (RAGGED) {
       const uint64_t v = ((static_cast<uint64_t>(q.y) << 32) | q.x) >> (8u * drop);
       q = make_uint2(static_cast<uint32_t>(v), static_cast<uint32_t>(v >> 32));
     }
     return q;
   }
   __device__ __forceinline__ void store_codes(Buffer b, uint2 q) const {
-    const uint32_t all = !ANY || n == V ? codes : kOutside;
+    const uint32_t all = !RAGGED || n == V ? codes : kOutside;
     if constexpr (V == 8) {
       const native_u2 t = {q.x, q.y};
       __builtin_amdgcn_raw_buffer_store_b64(t, b, all, 0, 0);
     } else {
       __builtin_amdgcn_raw_buffer_store_b32(q.x, b, all, 0, 0);
     }
-    if constexpr (ANY) {
+    if constexpr (RAGGED) {
       const uint32_t left = static_cast<uint32_t>(n < V ? n : 0), at = own(codes, 1);
       const uint32_t four = left & 4u, two = left & 2u;
       if constexpr (V == 8) __builtin_amdgcn_raw_buffer_store_b32(q.x, b, four ? at : kOutside, 0, 0);
@@ -242,18 +249,19 @@ template <int RPB> __device__ __forceinline__ uint32_t rows_in(int64_t base, int
 }
 
 // The second launch bound: waves per SIMD of the blocks a CU has at once.
-constexpr int bwd_bound(int vec, bool layer, bool post, bool pre, bool any, int tpr) {
-  return (bwd_blocks_per_cu(vec, layer, post, pre, any, tpr) * bwd_block(tpr) + 255) / 256;
+constexpr int bwd_bound(int vec, bool layer, bool post, bool pre, bool q8, int mode, int tpr) {
+  return (bwd_blocks_per_cu(vec, layer, post, pre, q8, mode, tpr) * bwd_block(tpr) + 255) / 256;
 }
 
 // Forward.  A block takes runs of rows (chunks) that share a gate row.
-template <typename T, bool LN, bool POST, bool PRE, bool COPY, bool ANY, int TPR>
+template <typename T, bool LN, bool POST, bool PRE, bool COPY, int MODE, int TPR>
 __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const StepArgs a) {
   constexpr int V = Tok<T>::VEC;
-  constexpr int BLOCK = fwd_block(TPR), RPB = BLOCK / TPR, D = fwd_depth(TPR, ANY);
+  constexpr bool OPTIONS = MODE == kAny;
+  constexpr int BLOCK = fwd_block(TPR), RPB = BLOCK / TPR, D = fwd_depth(TPR, MODE);
   __shared__ float lds[RowTotal<TPR, BLOCK, 1>::kFloats];
   int turn = 0;
-  const Place<T, TPR, BLOCK, ANY> pl(a);
+  const Place<T, TPR, BLOCK, MODE> pl(a);
   const uint32_t row_bytes = static_cast<uint32_t>(a.cols) * static_cast<uint32_t>(sizeof(T));
   const float inv = 1.f / static_cast<float>(a.cols);
   const uint32_t stat_out = threadIdx.x % TPR == 0 ? pl.stat : kOutside;
@@ -273,7 +281,7 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
       const uint32_t bytes = rows_in<RPB>(base, last) * row_bytes;
       x[u] = pl.load(buffer(a.x, off, bytes));
       r[u] = pl.load(buffer(a.res, off, bytes));
-      if constexpr (ANY) gf[u] = pl.load(buffer(a.gate_kind == 2 ? a.gate : nullptr, off, bytes));
+      if constexpr (OPTIONS) gf[u] = pl.load(buffer(a.gate_kind == 2 ? a.gate : nullptr, off, bytes));
     };
 #pragma unroll
     for (int u = 0; u < D; ++u) ask(u, first + u * RPB);
@@ -302,7 +310,7 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
       };
       if constexpr (COPY) copy(h, a.x8, a.x8_scale);
       float g[V];
-      if constexpr (ANY) {
+      if constexpr (OPTIONS) {
         Tok<T>::unpack(gf[u], g);
 #pragma unroll
         for (int j = 0; j < V; ++j) g[j] = a.gate_kind == 2 ? g[j] : 1.f;
@@ -323,10 +331,10 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           float d = LN ? h[j] - mean : h[j];
-          if constexpr (LN && ANY) d = j < pl.n ? d : 0.f;
+          if constexpr (LN && MODE != kWhole) d = j < pl.n ? d : 0.f;
           s[0] = fmaf(d, d, s[0]);
         }
-        if constexpr (LN && !ANY) s[0] = pl.n > 0 ? s[0] : 0.f;
+        if constexpr (LN && MODE == kWhole) s[0] = pl.n > 0 ? s[0] : 0.f;
         row_total<TPR, 1>(s, lds, turn);
         var = s[0] * inv;
       };
@@ -339,7 +347,7 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float xh = !(POST && LN) ? h[j] * rho : V == 8 ? fmaf(h[j], rho, shift1) : (h[j] - m1) * rho;
-        if constexpr (ANY) {
+        if constexpr (OPTIONS) {
           h[j] = fmaf(POST && LN ? fmaf(xh, kp[j], kb[j]) : xh * kp[j], g[j], q[j]);
         } else {
           if constexpr (POST && LN) q[j] += kb[j];
@@ -377,10 +385,10 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
 }
 
 // A kept tensor's vector as it was loaded: storage type, or an 8-bit copy.
-template <typename T, bool Q8, int TPR, int BLOCK, bool ANY> struct Kept {
+template <typename T, bool Q8, int TPR, int BLOCK, int MODE> struct Kept {
   Packed p;
   __device__ __forceinline__ void ask(const StepArgs &a, const void *data, const uint8_t *, int64_t base,
-                                      uint32_t rows, const Place<T, TPR, BLOCK, ANY> &pl) {
+                                      uint32_t rows, const Place<T, TPR, BLOCK, MODE> &pl) {
     p = pl.load(buffer(data, base * a.cols * static_cast<int64_t>(sizeof(T)),
                        rows * static_cast<uint32_t>(a.cols) * static_cast<uint32_t>(sizeof(T))));
   }
@@ -403,11 +411,11 @@ template <typename T, bool Q8, int TPR, int BLOCK, bool ANY> struct Kept {
     if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(p.v.x), "+v"(p.v.y), "+v"(p.v.z), "+v"(p.v.w));
   }
 };
-template <typename T, int TPR, int BLOCK, bool ANY> struct Kept<T, true, TPR, BLOCK, ANY> {
+template <typename T, int TPR, int BLOCK, int MODE> struct Kept<T, true, TPR, BLOCK, MODE> {
   uint2 q;
   uint32_t code;
   __device__ __forceinline__ void ask(const StepArgs &a, const void *data, const uint8_t *scales,
-                                      int64_t base, uint32_t rows, const Place<T, TPR, BLOCK, ANY> &pl) {
+                                      int64_t base, uint32_t rows, const Place<T, TPR, BLOCK, MODE> &pl) {
     q = pl.load_codes(buffer(data, base * a.cols, rows * static_cast<uint32_t>(a.cols)));
     code = __builtin_amdgcn_raw_buffer_load_b8(
         buffer(scales, base * a.groups8, rows * static_cast<uint32_t>(a.groups8)), pl.scale, 0, 0);
@@ -473,23 +481,24 @@ template <int V, int TPR> struct ColumnSum<V, TPR, true> {
 
 // Backward.  Each input vector is asked for again, for the next row, right
 // after its last use.
-template <typename T, bool LN, bool POST, bool PRE, bool Q8, bool ANY, int TPR>
-__global__ __launch_bounds__(bwd_block(TPR), bwd_bound(Tok<T>::VEC, LN, POST, PRE, ANY, TPR))
+template <typename T, bool LN, bool POST, bool PRE, bool Q8, int MODE, int TPR>
+__global__ __launch_bounds__(bwd_block(TPR), bwd_bound(Tok<T>::VEC, LN, POST, PRE, Q8, MODE, TPR))
 void step_bwd_rows_kernel(const StepArgs a) {
   constexpr int V = Tok<T>::VEC;
-  constexpr int BLOCK = bwd_block(TPR), RPB = BLOCK / TPR, D = bwd_depth(V, LN, POST, PRE, ANY, TPR);
+  constexpr bool OPTIONS = MODE == kAny;
+  constexpr int BLOCK = bwd_block(TPR), RPB = BLOCK / TPR, D = bwd_depth(V, LN, POST, PRE, Q8, MODE, TPR);
   constexpr int S = LN ? 2 : 1; // row sums per norm, column sums per norm
   __shared__ float lds[RowTotal<TPR, BLOCK, S>::kFloats];
   __shared__ float fold[RPB > 1 ? BLOCK * V : 1];
   int turn = 0;
-  const Place<T, TPR, BLOCK, ANY> pl(a);
+  const Place<T, TPR, BLOCK, MODE> pl(a);
   const uint32_t row_bytes = static_cast<uint32_t>(a.cols) * static_cast<uint32_t>(sizeof(T));
   const float inv = 1.f / static_cast<float>(a.cols);
   float kp[V], gn[V];
   // C, A: sums of gradient times normalized value; E, B: of the gradient (LN)
   constexpr bool TIGHT = TPR == 1024 && V == 8;
-  constexpr bool EB_LDS = LN && TIGHT, A_LDS = TIGHT && (ANY || (LN && Q8));
-  constexpr bool C_LDS = TIGHT && LN && (ANY || Q8);
+  constexpr bool EB_LDS = LN && TIGHT, A_LDS = TIGHT && (MODE != kWhole || (LN && Q8));
+  constexpr bool C_LDS = TIGHT && LN && (MODE != kWhole || Q8);
   __shared__ float4 eb_lds[EB_LDS ? 2 * TPR * V / 4 : 1], a_lds[A_LDS ? TPR * V / 4 : 1],
       c_lds[C_LDS ? TPR * V / 4 : 1];
   float4 *const e_lds = eb_lds, *const b_lds = eb_lds + (EB_LDS ? TPR * V / 4 : 0);
@@ -501,7 +510,7 @@ void step_bwd_rows_kernel(const StepArgs a) {
   E.clear(e_lds);
 
   struct Row {
-    Kept<T, Q8, TPR, BLOCK, ANY> x, h;
+    Kept<T, Q8, TPR, BLOCK, MODE> x, h;
     Packed dh, dy, gf;
     float m1, v1, m2, v2;
   } slot[D];
@@ -552,7 +561,7 @@ void step_bwd_rows_kernel(const StepArgs a) {
     auto ask_post = [&](Row &r, int64_t base) {
       const uint32_t rows = rows_in<RPB>(base, last);
       r.x.ask(a, a.x, a.kept_x_scale, base, rows, pl);
-      if constexpr (ANY)
+      if constexpr (OPTIONS)
         r.gf = pl.load(buffer(a.gate_kind == 2 ? a.gate : nullptr,
                             base * a.cols * static_cast<int64_t>(sizeof(T)), rows * row_bytes));
       if constexpr (POST) {
@@ -627,7 +636,7 @@ void step_bwd_rows_kernel(const StepArgs a) {
         r.x.template unit<LN>(a, mu, rho, xh);
       else
         r.x.get(a, xh);
-      if constexpr (ANY) {
+      if constexpr (OPTIONS) {
         const bool full = a.gate_kind == 2;
         float g[V];
         if constexpr (POST && LN) load_bias<V>(full ? a.beta_post : nullptr, pl.c, pl.n, g);
