@@ -54,13 +54,14 @@ struct StepPlan {
   bool layer = false, post = false, pre = false;
   bool kept8 = false;            // backward: x and h are 8-bit copies
   int mode = 0;                  // StepMode
-  int tpr = 0;                   // threads per row; 0: the kernels for long rows
+  int tpr = 0, nv = 0;           // layout; 0: the kernels for long rows
 };
 
-// Threads per row of the kernels that keep a row in registers, a 16-byte vector
-// each.
-#define NBLAHIP_STEP_LAYOUTS(CASE) \
-  CASE(16) CASE(32) CASE(64) CASE(128) CASE(192) CASE(256) CASE(384) CASE(512) CASE(640) CASE(768) CASE(1024)
+// Layouts of the kernels that keep a row in registers: threads per row, 16-byte
+// vectors per thread.
+#define NBLAHIP_STEP_LAYOUTS(CASE)                                                            \
+  CASE(16, 1) CASE(32, 1) CASE(64, 1) CASE(128, 1) CASE(192, 1) CASE(256, 1) CASE(384, 1)     \
+  CASE(512, 1) CASE(640, 1) CASE(768, 1) CASE(1024, 1) CASE(1024, 2)
 
 // Threads of a block.  Backward: 512 where a row takes 256 or fewer, so that the
 // rows of a block share one partial sum per column (half the partial sums of
@@ -69,8 +70,8 @@ constexpr int fwd_block(int tpr) { return tpr == 192 ? 192 : tpr < 256 ? 256 : t
 constexpr int bwd_block(int tpr) { return tpr == 192 ? 384 : tpr < 512 && tpr != 384 ? 512 : tpr; }
 
 // Backward: waves per SIMD that the registers of the row kernels allow (what the
-// compiler needs without a limit: 56 - 119 registers a thread, 76 - 148 with
-// `any`), and from them how many blocks a CU has at once: as many as are
+// compiler needs without a limit: 56 - 119 registers a thread, in the other forms
+// 76 - 148), and from them how many blocks a CU has at once: as many as are
 // launched, each walking its share of the rows.
 constexpr int bwd_waves(int vec, bool layer, bool post, bool pre, bool q8, int mode, int tpr) {
   const bool both = post && pre;
@@ -87,12 +88,40 @@ constexpr int bwd_blocks_per_cu(int vec, bool layer, bool post, bool pre, bool q
 // block, which otherwise stands still while its next row arrives ([8192, 8192]
 // bf16 175 -> 158 us), unless the registers of a block of 1024 are full; and in
 // the RMS step at two blocks ([8192, 4096] bf16 162 -> 159).
-constexpr int bwd_depth(int vec, bool layer, bool post, bool pre, bool q8, int mode, int tpr) {
+constexpr int bwd_depth(int vec, bool layer, bool post, bool pre, bool q8, int mode, int tpr, int nv) {
+  if (nv > 1) return 1;
   const bool full = tpr == 1024 && (vec == 8 ? mode != kWhole || (layer && post && pre) : mode != kWhole && layer);
   const int blocks = bwd_blocks_per_cu(vec, layer, post, pre, q8, mode, tpr);
   return (blocks == 1 && !full) || (blocks == 2 && vec == 8 && !layer && mode == kWhole && tpr == 512) ? 2 : 1;
 }
-constexpr int fwd_depth(int tpr, int mode) { return tpr >= 256 && !(mode != kWhole && tpr == 1024) ? 2 : 1; }
+constexpr int fwd_depth(int tpr, int nv, int mode) {
+  return tpr >= 256 && nv == 1 && !(mode != kWhole && tpr == 1024) ? 2 : 1;
+}
+// Column sums (C, A: of gradient times normalized value; E, B: of the gradient; C
+// and E of the second norm) that a block of 1024 threads keeps in LDS, at most
+// 128 KB, because its 128 registers a thread are taken.  w: columns of a
+// thread.
+enum { kSumC = 1, kSumE = 2, kSumA = 4, kSumB = 8 };
+constexpr unsigned bwd_sums_in_lds(int w, bool layer, bool post, bool pre, bool q8, int mode, int tpr) {
+  if (tpr != 1024 || w < 8) return 0;
+  if (w == 8)
+    return (layer ? kSumE | kSumB : 0) | (mode != kWhole || (layer && q8) ? kSumA : 0) |
+           (layer && (mode != kWhole || q8) ? kSumC : 0);
+  return kSumA; // (of 16 columns: the RMS norm alone, see bwd_row_fits)
+}
+// Forms that do not fit the registers (and LDS) of a block of 1024: they run as
+// long rows.
+constexpr bool bwd_row_fits(int vec, bool layer, bool post, bool pre, bool q8, int mode, int tpr, int nv) {
+  if (tpr < 1024) return true;
+  if (nv == 1) return !(vec == 8 && layer && post && pre && mode != kWhole);
+  if (vec == 8) return mode == kWhole && post && !pre && !layer;
+  return mode == kWhole ? !(layer && post && pre) : !(post && pre) && !(layer && pre && q8);
+}
+constexpr bool fwd_row_fits(int vec, bool layer, bool post, bool pre, bool copy, int mode, int nv) {
+  if (nv == 1) return true;
+  if (vec == 4) return !(layer && post && mode != kWhole);
+  return mode == kWhole && !(layer && post) && !(copy && pre);
+}
 
 int launch_step_fwd_f32(const StepPlan &pl, const StepArgs &a, hipStream_t st);
 int launch_step_fwd_f16(const StepPlan &pl, const StepArgs &a, hipStream_t st);

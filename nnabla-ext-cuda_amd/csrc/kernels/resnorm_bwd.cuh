@@ -10,23 +10,18 @@ namespace nblahip {
 
 template <typename T, bool LN, bool POST, bool PRE, bool Q8, int MODE>
 bool launch_bwd_rows(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
-  // the form that does not fit the registers of a block of 1024
-  // (step_bwd_is_long keeps it away)
-  constexpr int MOST = LN && POST && PRE && MODE != kWhole && sizeof(T) == 2 ? 768 : 1024;
-  switch (pl.tpr) {
-#define NBLAHIP_CASE(TPR)                                                                         \
-  case TPR:                                                                                       \
-    if constexpr (TPR <= MOST) {                                                                  \
+#define NBLAHIP_CASE(TPR, NV)                                                                     \
+  if (pl.tpr == TPR && pl.nv == NV) {                                                             \
+    if constexpr (bwd_row_fits(Tok<T>::VEC, LN, POST, PRE, Q8, MODE, TPR, NV) &&                  \
+                  !(NV > 1 && MODE == kRagged)) {                                                 \
       NBLAHIP_LAUNCH("step_bwd_rows_kernel",                                                      \
-                     (step_bwd_rows_kernel<T, LN, POST, PRE, Q8, MODE, TPR>),                      \
-                     dim3(static_cast<unsigned>(a.grid)), dim3(bwd_block(TPR)), 0, st, a);      \
+                     (step_bwd_rows_kernel<T, LN, POST, PRE, Q8, MODE, TPR, NV>),                 \
+                     dim3(static_cast<unsigned>(a.grid)), dim3(bwd_block(TPR)), 0, st, a);        \
       return true;                                                                                \
-    } else {                                                                                      \
-      return false;                                                                               \
-    }
-    NBLAHIP_STEP_LAYOUTS(NBLAHIP_CASE)
-#undef NBLAHIP_CASE
+    }                                                                                             \
   }
+  NBLAHIP_STEP_LAYOUTS(NBLAHIP_CASE)
+#undef NBLAHIP_CASE
   return false;
 }
 

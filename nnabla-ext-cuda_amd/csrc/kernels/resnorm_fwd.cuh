@@ -9,16 +9,17 @@ namespace nblahip {
 
 template <typename T, bool LN, bool POST, bool PRE, bool COPY, int MODE>
 bool launch_fwd_rows(const StepPlan &pl, const StepArgs &a, hipStream_t st) {
-  switch (pl.tpr) {
-#define NBLAHIP_CASE(TPR)                                                                         \
-  case TPR:                                                                                       \
-    NBLAHIP_LAUNCH("step_fwd_rows_kernel",                                                        \
-                   (step_fwd_rows_kernel<T, LN, POST, PRE, COPY, MODE, TPR>),                      \
-                   dim3(static_cast<unsigned>(a.grid)), dim3(fwd_block(TPR)), 0, st, a);        \
-    return true;
-    NBLAHIP_STEP_LAYOUTS(NBLAHIP_CASE)
-#undef NBLAHIP_CASE
+#define NBLAHIP_CASE(TPR, NV)                                                                     \
+  if (pl.tpr == TPR && pl.nv == NV) {                                                             \
+    if constexpr (fwd_row_fits(Tok<T>::VEC, LN, POST, PRE, COPY, MODE, NV) && !(NV > 1 && MODE == kRagged)) { \
+      NBLAHIP_LAUNCH("step_fwd_rows_kernel",                                                      \
+                     (step_fwd_rows_kernel<T, LN, POST, PRE, COPY, MODE, TPR, NV>),               \
+                     dim3(static_cast<unsigned>(a.grid)), dim3(fwd_block(TPR)), 0, st, a);        \
+      return true;                                                                                \
+    }                                                                                             \
   }
+  NBLAHIP_STEP_LAYOUTS(NBLAHIP_CASE)
+#undef NBLAHIP_CASE
   return false;
 }
 

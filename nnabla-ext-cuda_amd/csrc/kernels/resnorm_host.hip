@@ -64,16 +64,20 @@ constexpr int kCus = 256;
 
 int vec_of(int dtype) { return dtype == NBLAHIP_F32 ? 4 : 8; }
 
-// The layout with just enough threads for the row's vectors; longer rows,
-// and those of less than a vector, go to the kernels for long rows.
+// The layout with just enough threads for the row's vectors; rows longer than any
+// of them, and those of less than a vector, go to the kernels for long rows.
 void pick_layout(StepPlan &pl, int64_t cols) {
   const int64_t vec = vec_of(pl.dtype), vectors = (cols + vec - 1) / vec;
-  pl.tpr = 0;
+  pl.tpr = pl.nv = 0;
   if (cols < vec) return;
-#define NBLAHIP_CASE(TPR) \
-  if (pl.tpr == 0 && vectors <= TPR) pl.tpr = TPR;
+#define NBLAHIP_CASE(TPR, NV)             \
+  if (pl.tpr == 0 && vectors <= TPR * NV) { \
+    pl.tpr = TPR;                         \
+    pl.nv = NV;                           \
+  }
   NBLAHIP_STEP_LAYOUTS(NBLAHIP_CASE)
 #undef NBLAHIP_CASE
+  if (pl.nv > 1 && pl.mode == kRagged) pl.mode = kAny; // (one form for both)
 }
 
 // Whether every address that a 16-byte vector of the tensors (or its 8-bit
@@ -105,15 +109,11 @@ int64_t shared_gate_rows(const StepArgs &a, int64_t gate_rows) {
   return a.gate_kind == NBLAHIP_GATE_ROWS ? gate_rows : 1;
 }
 
-// The backward's only form whose rows of 1024 threads do not fit the registers.
-bool step_bwd_is_long(const StepPlan &pl) {
-  return pl.tpr == 1024 && pl.dtype != NBLAHIP_F32 && pl.layer && pl.post && pl.pre && pl.mode != kWhole;
-}
-
 // The backward's split, and its workspace laid out from `ws` (null: sizes only).
 size_t plan_bwd(StepArgs &a, StepPlan &pl, int64_t gate_rows, char *ws) {
   pick_layout(pl, a.cols);
-  if (step_bwd_is_long(pl)) pl.tpr = 0;
+  if (pl.tpr && !bwd_row_fits(vec_of(pl.dtype), pl.layer, pl.post, pl.pre, pl.kept8, pl.mode, pl.tpr, pl.nv))
+    pl.tpr = pl.nv = 0;
   a.pitch = (a.cols + 7) / 8 * 8;
   if (pl.tpr == 0) {
     plan_chunks(a, gate_rows, kCus, 16);
@@ -306,10 +306,12 @@ int step_fwd(StepArgs a, StepPlan pl, int64_t gate_rows, hipStream_t st) {
   al.write(a.x8_scale, qs);
   al.write(a.h8_scale, qs);
   if (al.bad()) return NBLAHIP_EALIAS;
-  pick_layout(pl, a.cols);
   pl.mode = a.gate_kind == NBLAHIP_GATE_FULL                                               ? kAny
             : whole_vectors(pl.dtype, a.cols, {a.x, a.res, a.h, a.y}, {a.x8, a.h8}) ? kWhole
                                                                                     : kRagged;
+  pick_layout(pl, a.cols);
+  if (pl.tpr && !fwd_row_fits(vec_of(pl.dtype), pl.layer, pl.post, pl.pre, a.x8 || a.h8, pl.mode, pl.nv))
+    pl.tpr = pl.nv = 0;
   gate_rows = shared_gate_rows(a, gate_rows);
   const int block = pl.tpr ? fwd_block(pl.tpr) : 1024;
   const int64_t blocks = kCus * (2048 / block);

@@ -1,5 +1,5 @@
-// The residual step on rows that fit a block at one 16-byte vector per thread:
-// every tensor crosses HBM once per direction.
+// The residual step on rows that fit a block at one or two 16-byte vectors per
+// thread: every tensor crosses HBM once per direction.
 //
 // TPR threads hold a row; a block takes several rows at a time where they are
 // short.  A thread's columns are the same in every row, so the
@@ -122,84 +122,131 @@ template <int N> __device__ __forceinline__ void settle(float (&v)[N]) {
   for (int j = 0; j < N; ++j) asm volatile("" : "+v"(v[j]));
 }
 
-// Where a thread's vector lies in the rows a block has in hand, in bytes from
+// Where a thread's NV vectors lie in the rows a block has in hand, in bytes from
 // the first of them: of a tensor of the storage type, of 8-bit codes, of their
 // scales, of a row statistic.  Of ragged rows the thread a row ends in reads the
 // vector `drop` elements further ahead, and writes the first `n` of its own.
-template <typename T, int TPR, int BLOCK, int MODE> struct Place {
-  static constexpr int V = Tok<T>::VEC;
+template <typename T, int TPR, int BLOCK, int MODE, int NV> struct Place {
+  static constexpr int V = Tok<T>::VEC, W = NV * V;
   static constexpr uint32_t SZ = sizeof(T);
   static constexpr bool RAGGED = MODE != kWhole;
-  uint32_t wide, codes, scale, stat;
-  uint32_t drop; // ragged rows only
-  int c, n;      // the thread's first column, and how many it has
+  struct Vec {
+    Packed p[NV];
+    // Hides the value from the optimiser, so that its widened form is made anew
+    // where it is needed instead of being kept in twice the registers.
+    __device__ __forceinline__ void pin() {
+      if constexpr (SZ == 2) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+          asm volatile("" : "+v"(p[k].v.x), "+v"(p[k].v.y), "+v"(p[k].v.z), "+v"(p[k].v.w));
+      }
+    }
+  };
+  uint32_t wide[NV], codes[NV], scale[NV], stat;
+  uint32_t drop[NV]; // ragged rows only
+  int n[NV];         // columns of the thread's
+  __device__ __forceinline__ static int first(int k) { // ... the first of them
+    return (k * TPR + static_cast<int>(threadIdx.x % TPR)) * V;
+  }
   __device__ __forceinline__ Place(const StepArgs &a) {
     const uint32_t cols = static_cast<uint32_t>(a.cols);
     const uint32_t sub = BLOCK == TPR ? 0 : threadIdx.x / TPR;
-    c = (threadIdx.x % TPR) * V;
-    n = columns_left(a.cols - c, V);
-    drop = RAGGED && n > 0 ? V - n : 0;
-    wide = n > 0 ? (sub * cols + c - drop) * SZ : kOutside;
-    codes = n > 0 ? sub * cols + c - drop : kOutside;
-    scale = n > 0 ? sub * static_cast<uint32_t>(a.groups8) + c / kAct8Group : kOutside;
     stat = sub * 4;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = first(k);
+      n[k] = columns_left(a.cols - c, V);
+      drop[k] = RAGGED && n[k] > 0 ? V - n[k] : 0;
+      wide[k] = n[k] > 0 ? (sub * cols + c - drop[k]) * SZ : kOutside;
+      codes[k] = n[k] > 0 ? sub * cols + c - drop[k] : kOutside;
+      scale[k] = n[k] > 0 ? sub * static_cast<uint32_t>(a.groups8) + c / kAct8Group : kOutside;
+    }
   }
-  __device__ __forceinline__ Packed load(Buffer b) const {
-    Packed r = buffer_load(b, wide);
-    if constexpr (RAGGED) r.v = shift_down_bits(r.v, drop * 8u * SZ);
+  // whether element j of the thread's W is a column of the row
+  __device__ __forceinline__ bool has(int j) const { return j % V < n[j / V]; }
+  __device__ __forceinline__ void param(const float *p, float (&o)[W]) const {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) load_param<V>(p, first(k), n[k], reinterpret_cast<float(&)[V]>(o[k * V]));
+  }
+  __device__ __forceinline__ void bias(const float *p, float (&o)[W]) const {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) load_bias<V>(p, first(k), n[k], reinterpret_cast<float(&)[V]>(o[k * V]));
+  }
+  __device__ __forceinline__ static void unpack(const Vec &r, float (&o)[W]) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) Tok<T>::unpack(r.p[k], reinterpret_cast<float(&)[V]>(o[k * V]));
+  }
+  __device__ __forceinline__ static Vec pack(const float (&o)[W]) {
+    Vec r;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) r.p[k] = Tok<T>::pack(reinterpret_cast<const float(&)[V]>(o[k * V]));
     return r;
   }
-  // Offsets of the pieces a vector that is cut short is written in.
-  __device__ __forceinline__ uint32_t own(uint32_t at, uint32_t size) const {
-    return n > 0 ? at + drop * size : kOutside;
+  __device__ __forceinline__ Vec load(Buffer b) const {
+    Vec r;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      r.p[k] = buffer_load(b, wide[k]);
+      if constexpr (RAGGED) r.p[k].v = shift_down_bits(r.p[k].v, drop[k] * 8u * SZ);
+    }
+    return r;
   }
-  __device__ __forceinline__ void store(Buffer b, const Packed &r) const {
-    if constexpr (!RAGGED) {
-      buffer_store(b, wide, r);
-    } else {
-      buffer_store(b, n == V ? wide : kOutside, r);
-      const uint32_t left = static_cast<uint32_t>(n < V ? n : 0); // elements still to write
-      const uint32_t at = own(wide, SZ);
-      const uint32_t four = left & (8 / SZ), two = left & (4 / SZ);
-      const native_u2 t = {r.v.x, r.v.y};
-      __builtin_amdgcn_raw_buffer_store_b64(t, b, four ? at : kOutside, 0, 0);
-      const uint4 q = shift_down_bits(r.v, four ? 64u : 0u);
-      __builtin_amdgcn_raw_buffer_store_b32(q.x, b, two ? at + four * SZ : kOutside, 0, 0);
-      if constexpr (SZ == 2) {
-        const uint32_t w = two ? q.y : q.x;
-        __builtin_amdgcn_raw_buffer_store_b16(static_cast<uint16_t>(w), b,
-                                              left & 1u ? at + (four + two) * SZ : kOutside, 0, 0);
+  // Offset of the first of the thread's own elements, where it starts to write
+  // the pieces of a vector that is cut short.
+  __device__ __forceinline__ uint32_t own(uint32_t at, int k, uint32_t size) const {
+    return n[k] > 0 ? at + drop[k] * size : kOutside;
+  }
+  __device__ __forceinline__ void store(Buffer b, const Vec &r) const {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if constexpr (!RAGGED) {
+        buffer_store(b, wide[k], r.p[k]);
+      } else {
+        const uint4 v = r.p[k].v;
+        buffer_store(b, n[k] == V ? wide[k] : kOutside, r.p[k]);
+        const uint32_t left = static_cast<uint32_t>(n[k] < V ? n[k] : 0); // elements still to write
+        const uint32_t at = own(wide[k], k, SZ);
+        const uint32_t four = left & (8 / SZ), two = left & (4 / SZ);
+        const native_u2 t = {v.x, v.y};
+        __builtin_amdgcn_raw_buffer_store_b64(t, b, four ? at : kOutside, 0, 0);
+        const uint4 q = shift_down_bits(v, four ? 64u : 0u);
+        __builtin_amdgcn_raw_buffer_store_b32(q.x, b, two ? at + four * SZ : kOutside, 0, 0);
+        if constexpr (SZ == 2) {
+          const uint32_t w = two ? q.y : q.x;
+          __builtin_amdgcn_raw_buffer_store_b16(static_cast<uint16_t>(w), b,
+                                                left & 1u ? at + (four + two) * SZ : kOutside, 0, 0);
+        }
       }
     }
   }
   // onto what `old` (a buffer without records: nothing) holds there
-  __device__ __forceinline__ void put(Buffer b, Buffer old, const float (&o)[V]) const {
+  __device__ __forceinline__ void put(Buffer b, Buffer old, const float (&o)[W]) const {
     if constexpr (MODE == kAny) {
-      float sum[V];
-      Tok<T>::unpack(load(old), sum);
+      float sum[W];
+      unpack(load(old), sum);
 #pragma unroll
-      for (int j = 0; j < V; ++j) sum[j] += o[j];
-      store(b, Tok<T>::pack(sum));
+      for (int j = 0; j < W; ++j) sum[j] += o[j];
+      store(b, pack(sum));
     } else {
-      store(b, Tok<T>::pack(o));
+      store(b, pack(o));
     }
   }
-  __device__ __forceinline__ uint2 load_codes(Buffer b) const {
+  __device__ __forceinline__ uint2 load_codes(Buffer b, int k) const {
     uint2 q = make_uint2(0u, 0u);
     if constexpr (V == 8) {
-      const native_u2 t = __builtin_amdgcn_raw_buffer_load_b64(b, codes, 0, 0);
+      const native_u2 t = __builtin_amdgcn_raw_buffer_load_b64(b, codes[k], 0, 0);
       q = make_uint2(t.x, t.y);
     } else {
-      q.x = __builtin_amdgcn_raw_buffer_load_b32(b, codes, 0, 0);
+      q.x = __builtin_amdgcn_raw_buffer_load_b32(b, codes[k], 0, 0);
     }
     if constexpr (RAGGED) {
-      const uint64_t v = ((static_cast<uint64_t>(q.y) << 32) | q.x) >> (8u * drop);
+      const uint64_t v = ((static_cast<uint64_t>(q.y) << 32) | q.x) >> (8u * drop[k]);
       q = make_uint2(static_cast<uint32_t>(v), static_cast<uint32_t>(v >> 32));
     }
     return q;
   }
-  __device__ __forceinline__ void store_codes(Buffer b, uint2 q) const {
-    const uint32_t all = !RAGGED || n == V ? codes : kOutside;
+  __device__ __forceinline__ void store_codes(Buffer b, uint2 q, int k) const {
+    const uint32_t all = !RAGGED || n[k] == V ? codes[k] : kOutside;
     if constexpr (V == 8) {
       const native_u2 t = {q.x, q.y};
       __builtin_amdgcn_raw_buffer_store_b64(t, b, all, 0, 0);
@@ -207,7 +254,7 @@ template <typename T, int TPR, int BLOCK, int MODE> struct Place {
       __builtin_amdgcn_raw_buffer_store_b32(q.x, b, all, 0, 0);
     }
     if constexpr (RAGGED) {
-      const uint32_t left = static_cast<uint32_t>(n < V ? n : 0), at = own(codes, 1);
+      const uint32_t left = static_cast<uint32_t>(n[k] < V ? n[k] : 0), at = own(codes[k], k, 1);
       const uint32_t four = left & 4u, two = left & 2u;
       if constexpr (V == 8) __builtin_amdgcn_raw_buffer_store_b32(q.x, b, four ? at : kOutside, 0, 0);
       const uint32_t w = four ? q.y : q.x;
@@ -221,25 +268,22 @@ template <typename T, int TPR, int BLOCK, int MODE> struct Place {
 // The factor between the normalized x and its part of h, branch_scale * gate *
 // gamma_post (without a norm: branch_scale * gate), at a thread's columns, and
 // the same of beta_post.  A gate per element comes in later.
-template <int V, bool POST>
-__device__ __forceinline__ void load_branch(const StepArgs &a, int64_t gate_row, int64_t c, int n,
-                                            float (&k)[V]) {
-  float g[V];
-  load_param<V>(POST ? a.gamma_post : nullptr, c, n, k);
-  load_param<V>(a.gate_kind == 1 ? static_cast<const float *>(a.gate) + gate_row * a.cols : nullptr, c,
-                n, g);
+template <bool POST, typename P>
+__device__ __forceinline__ void load_branch(const StepArgs &a, int64_t gate_row, const P &pl, float (&k)[P::W]) {
+  float g[P::W];
+  pl.param(POST ? a.gamma_post : nullptr, k);
+  pl.param(a.gate_kind == 1 ? static_cast<const float *>(a.gate) + gate_row * a.cols : nullptr, g);
 #pragma unroll
-  for (int j = 0; j < V; ++j) k[j] *= a.branch_scale * g[j];
+  for (int j = 0; j < P::W; ++j) k[j] *= a.branch_scale * g[j];
 }
-template <int V>
-__device__ __forceinline__ void load_branch_bias(const StepArgs &a, int64_t gate_row, int64_t c, int n,
-                                                 float (&k)[V]) {
-  float g[V];
-  load_bias<V>(a.beta_post, c, n, k);
-  load_param<V>(a.gate_kind == 1 ? static_cast<const float *>(a.gate) + gate_row * a.cols : nullptr, c,
-                n, g);
+template <typename P>
+__device__ __forceinline__ void load_branch_bias(const StepArgs &a, int64_t gate_row, const P &pl,
+                                                 float (&k)[P::W]) {
+  float g[P::W];
+  pl.bias(a.beta_post, k);
+  pl.param(a.gate_kind == 1 ? static_cast<const float *>(a.gate) + gate_row * a.cols : nullptr, g);
 #pragma unroll
-  for (int j = 0; j < V; ++j) k[j] *= a.branch_scale * g[j];
+  for (int j = 0; j < P::W; ++j) k[j] *= a.branch_scale * g[j];
 }
 
 // Rows of [base, base + RPB) that lie before `last`.
@@ -249,33 +293,34 @@ template <int RPB> __device__ __forceinline__ uint32_t rows_in(int64_t base, int
 }
 
 // The second launch bound: waves per SIMD of the blocks a CU has at once.
-constexpr int bwd_bound(int vec, bool layer, bool post, bool pre, bool q8, int mode, int tpr) {
+constexpr int bwd_bound(int vec, bool layer, bool post, bool pre, bool q8, int mode, int tpr, int nv) {
   return (bwd_blocks_per_cu(vec, layer, post, pre, q8, mode, tpr) * bwd_block(tpr) + 255) / 256;
 }
 
 // Forward.  A block takes runs of rows (chunks) that share a gate row.
-template <typename T, bool LN, bool POST, bool PRE, bool COPY, int MODE, int TPR>
+template <typename T, bool LN, bool POST, bool PRE, bool COPY, int MODE, int TPR, int NV>
 __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const StepArgs a) {
-  constexpr int V = Tok<T>::VEC;
+  using P = Place<T, TPR, fwd_block(TPR), MODE, NV>;
+  using Vec = typename P::Vec;
+  constexpr int V = P::V, W = P::W;
   constexpr bool OPTIONS = MODE == kAny;
-  constexpr int BLOCK = fwd_block(TPR), RPB = BLOCK / TPR, D = fwd_depth(TPR, MODE);
+  constexpr int BLOCK = fwd_block(TPR), RPB = BLOCK / TPR, D = fwd_depth(TPR, NV, MODE);
   __shared__ float lds[RowTotal<TPR, BLOCK, 1>::kFloats];
   int turn = 0;
-  const Place<T, TPR, BLOCK, MODE> pl(a);
+  const P pl(a);
   const uint32_t row_bytes = static_cast<uint32_t>(a.cols) * static_cast<uint32_t>(sizeof(T));
   const float inv = 1.f / static_cast<float>(a.cols);
   const uint32_t stat_out = threadIdx.x % TPR == 0 ? pl.stat : kOutside;
-  const uint32_t scale_out = pl.c % kAct8Group == 0 ? pl.scale : kOutside;
-  float gn[V], bn[V], kp[V], kb[V];
-  if constexpr (PRE) load_param<V>(a.gamma_pre, pl.c, pl.n, gn);
-  if constexpr (PRE && LN) load_bias<V>(a.beta_pre, pl.c, pl.n, bn);
+  float gn[W], bn[W], kp[W], kb[W];
+  if constexpr (PRE) pl.param(a.gamma_pre, gn);
+  if constexpr (PRE && LN) pl.bias(a.beta_pre, bn);
   for (int64_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
     const int64_t group = chunk / a.chunks_per_gate;
     const int64_t first = group * a.rows_per_gate + chunk % a.chunks_per_gate * a.chunk_rows;
     const int64_t last = least(first + a.chunk_rows, (group + 1) * a.rows_per_gate);
-    load_branch<V, POST>(a, group, pl.c, pl.n, kp);
-    if constexpr (POST && LN) load_branch_bias<V>(a, group, pl.c, pl.n, kb);
-    Packed x[D], r[D], gf[D];
+    load_branch<POST>(a, group, pl, kp);
+    if constexpr (POST && LN) load_branch_bias(a, group, pl, kb);
+    Vec x[D], r[D], gf[D];
     auto ask = [&](int u, int64_t base) {
       const int64_t off = base * a.cols * static_cast<int64_t>(sizeof(T));
       const uint32_t bytes = rows_in<RPB>(base, last) * row_bytes;
@@ -293,27 +338,29 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
       if (u > 0 && base >= last) break;
       const uint32_t rows = rows_in<RPB>(base, last), bytes = rows * row_bytes;
       const int64_t off = base * a.cols * static_cast<int64_t>(sizeof(T));
-      float h[V], q[V];
+      float h[W], q[W];
       float m1 = 0.f, v1 = 0.f, m2 = 0.f, v2 = 0.f;
-      Tok<T>::unpack(x[u], h);
-      Tok<T>::unpack(r[u], q);
+      P::unpack(x[u], h);
+      P::unpack(r[u], q);
 #pragma unroll
-      for (int j = 0; j < V; ++j) q[j] *= a.res_scale;
-      auto copy = [&](const float (&v)[V], void *codes, void *scales) {
-        uint32_t code;
-        const uint2 w = act8_encode<V>(v, a.format8, code);
+      for (int j = 0; j < W; ++j) q[j] *= a.res_scale;
+      auto copy = [&](const float (&v)[W], void *codes, void *scales) {
         const Buffer to = buffer(codes, base * a.cols, rows * static_cast<uint32_t>(a.cols));
-        pl.store_codes(to, w);
-        __builtin_amdgcn_raw_buffer_store_b8(
-            static_cast<uint8_t>(code),
-            buffer(scales, base * a.groups8, rows * static_cast<uint32_t>(a.groups8)), scale_out, 0, 0);
+        const Buffer of = buffer(scales, base * a.groups8, rows * static_cast<uint32_t>(a.groups8));
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          uint32_t code;
+          pl.store_codes(to, act8_encode<V>(reinterpret_cast<const float(&)[V]>(v[k * V]), a.format8, code), k);
+          __builtin_amdgcn_raw_buffer_store_b8(static_cast<uint8_t>(code), of,
+                                               P::first(k) % kAct8Group == 0 ? pl.scale[k] : kOutside, 0, 0);
+        }
       };
       if constexpr (COPY) copy(h, a.x8, a.x8_scale);
-      float g[V];
+      float g[W];
       if constexpr (OPTIONS) {
-        Tok<T>::unpack(gf[u], g);
+        P::unpack(gf[u], g);
 #pragma unroll
-        for (int j = 0; j < V; ++j) g[j] = a.gate_kind == 2 ? g[j] : 1.f;
+        for (int j = 0; j < W; ++j) g[j] = a.gate_kind == 2 ? g[j] : 1.f;
         settle(g);
       }
       settle(h);
@@ -323,18 +370,18 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
         float s[1] = {0.f};
         if constexpr (LN) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) s[0] += h[j];
+          for (int j = 0; j < W; ++j) s[0] += h[j];
           row_total<TPR, 1>(s, lds, turn);
           mean = s[0] * inv;
         }
         s[0] = 0.f;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
+        for (int j = 0; j < W; ++j) {
           float d = LN ? h[j] - mean : h[j];
-          if constexpr (LN && MODE != kWhole) d = j < pl.n ? d : 0.f;
+          if constexpr (LN && (MODE != kWhole || NV > 1)) d = pl.has(j) ? d : 0.f;
           s[0] = fmaf(d, d, s[0]);
         }
-        if constexpr (LN && MODE == kWhole) s[0] = pl.n > 0 ? s[0] : 0.f;
+        if constexpr (LN && MODE == kWhole && NV == 1) s[0] = pl.n[0] > 0 ? s[0] : 0.f;
         row_total<TPR, 1>(s, lds, turn);
         var = s[0] * inv;
       };
@@ -345,7 +392,7 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
       }
       const float shift1 = -m1 * rho; // 16-bit data: see Kept::unit
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
+      for (int j = 0; j < W; ++j) {
         const float xh = !(POST && LN) ? h[j] * rho : V == 8 ? fmaf(h[j], rho, shift1) : (h[j] - m1) * rho;
         if constexpr (OPTIONS) {
           h[j] = fmaf(POST && LN ? fmaf(xh, kp[j], kb[j]) : xh * kp[j], g[j], q[j]);
@@ -354,22 +401,22 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
           h[j] = fmaf(xh, kp[j], q[j]);
         }
       }
-      const Packed hp = Tok<T>::pack(h);
+      const Vec hp = P::pack(h);
       pl.store(buffer(a.h, off, bytes), hp);
       if constexpr (COPY && PRE) {
-        float hv[V];
-        Tok<T>::unpack(hp, hv);
+        float hv[W];
+        P::unpack(hp, hv);
         copy(hv, a.h8, a.h8_scale);
       }
       if constexpr (PRE) {
         moments(m2, v2);
         const float rho2 = inv_std(v2, a.eps), shift2 = -m2 * rho2;
-        float y[V];
+        float y[W];
 #pragma unroll
-        for (int j = 0; j < V; ++j)
+        for (int j = 0; j < W; ++j)
           y[j] = !LN ? h[j] * rho2 * gn[j]
                      : fmaf(V == 8 ? fmaf(h[j], rho2, shift2) : (h[j] - m2) * rho2, gn[j], bn[j]);
-        pl.store(buffer(a.y, off, bytes), Tok<T>::pack(y));
+        pl.store(buffer(a.y, off, bytes), P::pack(y));
       }
       if constexpr (POST) {
         if constexpr (LN) buffer_store_float(buffer(a.mean_post, 4 * base, 4 * rows), stat_out, m1);
@@ -384,82 +431,91 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
   }
 }
 
-// A kept tensor's vector as it was loaded: storage type, or an 8-bit copy.
-template <typename T, bool Q8, int TPR, int BLOCK, int MODE> struct Kept {
-  Packed p;
+// A kept tensor's vectors as they were loaded: storage type, or an 8-bit copy.
+template <typename T, bool Q8, typename P> struct Kept {
+  static constexpr int W = P::W;
+  typename P::Vec p;
   __device__ __forceinline__ void ask(const StepArgs &a, const void *data, const uint8_t *, int64_t base,
-                                      uint32_t rows, const Place<T, TPR, BLOCK, MODE> &pl) {
+                                      uint32_t rows, const P &pl) {
     p = pl.load(buffer(data, base * a.cols * static_cast<int64_t>(sizeof(T)),
                        rows * static_cast<uint32_t>(a.cols) * static_cast<uint32_t>(sizeof(T))));
   }
-  __device__ __forceinline__ void get(const StepArgs &, float (&o)[Tok<T>::VEC]) const {
-    Tok<T>::unpack(p, o);
-  }
+  __device__ __forceinline__ void get(const StepArgs &, float (&o)[W]) const { P::unpack(p, o); }
   // (value - mu) * rho.  16-bit data takes one fma, value * rho - mu * rho: off by
   // 2^-24 |mu| rho, far below what the data resolves; float data is centred first.
   template <bool CENTRED>
-  __device__ __forceinline__ void unit(const StepArgs &a, float mu, float rho, float (&o)[Tok<T>::VEC]) const {
+  __device__ __forceinline__ void unit(const StepArgs &a, float mu, float rho, float (&o)[W]) const {
     get(a, o);
     const float shift = -mu * rho;
 #pragma unroll
-    for (int j = 0; j < Tok<T>::VEC; ++j)
+    for (int j = 0; j < W; ++j)
       o[j] = !CENTRED ? o[j] * rho : sizeof(T) == 2 ? fmaf(o[j], rho, shift) : (o[j] - mu) * rho;
   }
-  // Hides the value from the optimiser, so that its widened form is made anew
-  // where it is needed instead of being kept in twice the registers.
-  __device__ __forceinline__ void pin() {
-    if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(p.v.x), "+v"(p.v.y), "+v"(p.v.z), "+v"(p.v.w));
-  }
+  __device__ __forceinline__ void pin() { p.pin(); }
 };
-template <typename T, int TPR, int BLOCK, int MODE> struct Kept<T, true, TPR, BLOCK, MODE> {
-  uint2 q;
-  uint32_t code;
+template <typename T, typename P> struct Kept<T, true, P> {
+  static constexpr int W = P::W, V = P::V, NV = W / V;
+  uint2 q[NV];
+  uint32_t code[NV];
   __device__ __forceinline__ void ask(const StepArgs &a, const void *data, const uint8_t *scales,
-                                      int64_t base, uint32_t rows, const Place<T, TPR, BLOCK, MODE> &pl) {
-    q = pl.load_codes(buffer(data, base * a.cols, rows * static_cast<uint32_t>(a.cols)));
-    code = __builtin_amdgcn_raw_buffer_load_b8(
-        buffer(scales, base * a.groups8, rows * static_cast<uint32_t>(a.groups8)), pl.scale, 0, 0);
+                                      int64_t base, uint32_t rows, const P &pl) {
+    const Buffer codes = buffer(data, base * a.cols, rows * static_cast<uint32_t>(a.cols));
+    const Buffer of = buffer(scales, base * a.groups8, rows * static_cast<uint32_t>(a.groups8));
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      q[k] = pl.load_codes(codes, k);
+      code[k] = __builtin_amdgcn_raw_buffer_load_b8(of, pl.scale[k], 0, 0);
+    }
   }
-  __device__ __forceinline__ void get(const StepArgs &a, float (&o)[Tok<T>::VEC]) const {
-    act8_decode<Tok<T>::VEC>(q, code, a.format8, o);
+  __device__ __forceinline__ void get(const StepArgs &a, float (&o)[W]) const {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      act8_decode<V>(q[k], code[k], a.format8, reinterpret_cast<float(&)[V]>(o[k * V]));
   }
   // One multiplication takes the scale (a power of two: exact) and rho.
   template <bool CENTRED>
-  __device__ __forceinline__ void unit(const StepArgs &a, float mu, float rho, float (&o)[Tok<T>::VEC]) const {
-    const float scale = act8_scale(code) * rho, shift = -mu * rho;
-    act8_numbers<Tok<T>::VEC>(q, a.format8, o);
+  __device__ __forceinline__ void unit(const StepArgs &a, float mu, float rho, float (&o)[W]) const {
+    const float shift = -mu * rho;
 #pragma unroll
-    for (int j = 0; j < Tok<T>::VEC; ++j) o[j] = CENTRED ? fmaf(o[j], scale, shift) : o[j] * scale;
+    for (int k = 0; k < NV; ++k) {
+      const float scale = act8_scale(code[k]) * rho;
+      act8_numbers<V>(q[k], a.format8, reinterpret_cast<float(&)[V]>(o[k * V]));
+#pragma unroll
+      for (int j = k * V; j < (k + 1) * V; ++j) o[j] = CENTRED ? fmaf(o[j], scale, shift) : o[j] * scale;
+    }
   }
-  __device__ __forceinline__ void pin() { asm volatile("" : "+v"(q.x), "+v"(q.y), "+v"(code)); }
+  __device__ __forceinline__ void pin() {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) asm volatile("" : "+v"(q[k].x), "+v"(q[k].y), "+v"(code[k]));
+  }
 };
 
 // Column sums of one kind for the thread's columns: in registers, or in LDS where
 // a block of 1024 threads has none left for them (16 bytes of LDS traffic per
-// column and row against 24 of HBM's for the whole CU: it does not show).
-template <int V, int TPR, bool IN_LDS> struct ColumnSum {
-  float v[V];
+// column and row beside 12 of HBM's, at ten times its rate: it does not show).
+template <int W, int TPR, bool IN_LDS> struct ColumnSum {
+  float v[W];
   __device__ __forceinline__ void clear(float4 *) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = 0.f;
+    for (int j = 0; j < W; ++j) v[j] = 0.f;
   }
   __device__ __forceinline__ void add(float4 *, int j, float a, float b) { v[j] = fmaf(a, b, v[j]); }
   __device__ __forceinline__ void load(float4 *) {}
   __device__ __forceinline__ void save(float4 *) { settle(v); }
-  __device__ __forceinline__ void get(const float4 *, float (&o)[V]) const {
+  __device__ __forceinline__ void get(const float4 *, float (&o)[W]) const {
 #pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = v[j];
+    for (int j = 0; j < W; ++j) o[j] = v[j];
   }
 };
-template <int V, int TPR> struct ColumnSum<V, TPR, true> {
-  float v[V]; // only between load and save
+template <int W, int TPR> struct ColumnSum<W, TPR, true> {
+  float v[W]; // only between load and save
   __device__ __forceinline__ void clear(float4 *lds) {
 #pragma unroll
-    for (int j = 0; j < V / 4; ++j) lds[j * TPR + threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = 0; j < W / 4; ++j) lds[j * TPR + threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   __device__ __forceinline__ void load(float4 *lds) {
 #pragma unroll
-    for (int j = 0; j < V / 4; ++j) {
+    for (int j = 0; j < W / 4; ++j) {
       const float4 t = lds[j * TPR + threadIdx.x];
       v[4 * j] = t.x; v[4 * j + 1] = t.y; v[4 * j + 2] = t.z; v[4 * j + 3] = t.w;
     }
@@ -467,12 +523,12 @@ template <int V, int TPR> struct ColumnSum<V, TPR, true> {
   __device__ __forceinline__ void add(float4 *, int j, float a, float b) { v[j] = fmaf(a, b, v[j]); }
   __device__ __forceinline__ void save(float4 *lds) {
 #pragma unroll
-    for (int j = 0; j < V / 4; ++j)
+    for (int j = 0; j < W / 4; ++j)
       lds[j * TPR + threadIdx.x] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
   }
-  __device__ __forceinline__ void get(const float4 *lds, float (&o)[V]) const {
+  __device__ __forceinline__ void get(const float4 *lds, float (&o)[W]) const {
 #pragma unroll
-    for (int j = 0; j < V / 4; ++j) {
+    for (int j = 0; j < W / 4; ++j) {
       const float4 t = lds[j * TPR + threadIdx.x];
       o[4 * j] = t.x; o[4 * j + 1] = t.y; o[4 * j + 2] = t.z; o[4 * j + 3] = t.w;
     }
@@ -481,48 +537,53 @@ template <int V, int TPR> struct ColumnSum<V, TPR, true> {
 
 // Backward.  Each input vector is asked for again, for the next row, right
 // after its last use.
-template <typename T, bool LN, bool POST, bool PRE, bool Q8, int MODE, int TPR>
-__global__ __launch_bounds__(bwd_block(TPR), bwd_bound(Tok<T>::VEC, LN, POST, PRE, Q8, MODE, TPR))
+template <typename T, bool LN, bool POST, bool PRE, bool Q8, int MODE, int TPR, int NV>
+__global__ __launch_bounds__(bwd_block(TPR), bwd_bound(Tok<T>::VEC, LN, POST, PRE, Q8, MODE, TPR, NV))
 void step_bwd_rows_kernel(const StepArgs a) {
-  constexpr int V = Tok<T>::VEC;
+  using P = Place<T, TPR, bwd_block(TPR), MODE, NV>;
+  using Vec = typename P::Vec;
+  constexpr int V = P::V, W = P::W;
   constexpr bool OPTIONS = MODE == kAny;
-  constexpr int BLOCK = bwd_block(TPR), RPB = BLOCK / TPR, D = bwd_depth(V, LN, POST, PRE, Q8, MODE, TPR);
+  constexpr int BLOCK = bwd_block(TPR), RPB = BLOCK / TPR, D = bwd_depth(V, LN, POST, PRE, Q8, MODE, TPR, NV);
   constexpr int S = LN ? 2 : 1; // row sums per norm, column sums per norm
   __shared__ float lds[RowTotal<TPR, BLOCK, S>::kFloats];
   __shared__ float fold[RPB > 1 ? BLOCK * V : 1];
   int turn = 0;
-  const Place<T, TPR, BLOCK, MODE> pl(a);
+  const P pl(a);
   const uint32_t row_bytes = static_cast<uint32_t>(a.cols) * static_cast<uint32_t>(sizeof(T));
   const float inv = 1.f / static_cast<float>(a.cols);
-  float kp[V], gn[V];
+  float kp[W], gn[W];
   // C, A: sums of gradient times normalized value; E, B: of the gradient (LN)
-  constexpr bool TIGHT = TPR == 1024 && V == 8;
-  constexpr bool EB_LDS = LN && TIGHT, A_LDS = TIGHT && (MODE != kWhole || (LN && Q8));
-  constexpr bool C_LDS = TIGHT && LN && (MODE != kWhole || Q8);
-  __shared__ float4 eb_lds[EB_LDS ? 2 * TPR * V / 4 : 1], a_lds[A_LDS ? TPR * V / 4 : 1],
-      c_lds[C_LDS ? TPR * V / 4 : 1];
-  float4 *const e_lds = eb_lds, *const b_lds = eb_lds + (EB_LDS ? TPR * V / 4 : 0);
-  ColumnSum<V, TPR, C_LDS> C;
-  ColumnSum<V, TPR, EB_LDS> E, B;
-  ColumnSum<V, TPR, A_LDS> A;
-  if constexpr (PRE) load_param<V>(a.gamma_pre, pl.c, pl.n, gn);
+  // (which of them are in LDS: bwd_sums_in_lds)
+  constexpr unsigned IN = bwd_sums_in_lds(W, LN, POST, PRE, Q8, MODE, TPR);
+  constexpr int F4 = TPR * W / 4;
+  __shared__ float4 c_lds[IN & kSumC ? F4 : 1], e_lds[IN & kSumE ? F4 : 1], a_lds[IN & kSumA ? F4 : 1],
+      b_lds[IN & kSumB ? F4 : 1];
+  ColumnSum<W, TPR, (IN & kSumC) != 0> C;
+  ColumnSum<W, TPR, (IN & kSumE) != 0> E;
+  ColumnSum<W, TPR, (IN & kSumA) != 0> A;
+  ColumnSum<W, TPR, (IN & kSumB) != 0> B;
+  if constexpr (PRE) pl.param(a.gamma_pre, gn);
   C.clear(c_lds);
   E.clear(e_lds);
 
   struct Row {
-    Kept<T, Q8, TPR, BLOCK, MODE> x, h;
-    Packed dh, dy, gf;
+    Kept<T, Q8, P> x, h;
+    Vec dh, dy, gf;
     float m1, v1, m2, v2;
   } slot[D];
   // Column sums (times `scale`) of the block's rows-at-a-time to `out`; every
   // thread of the block is here.
-  auto flush = [&](float *out, const float (&s)[V], float scale) {
+  auto flush = [&](float *out, const float (&s)[W], float scale) {
     if constexpr (RPB == 1) {
-      if (pl.c < a.pitch) {
 #pragma unroll
-        for (int j = 0; j < V; j += 4)
-          *reinterpret_cast<float4 *>(out + pl.c + j) =
-              make_float4(s[j] * scale, s[j + 1] * scale, s[j + 2] * scale, s[j + 3] * scale);
+      for (int k = 0; k < NV; ++k) {
+        if (P::first(k) < a.pitch) {
+#pragma unroll
+          for (int j = k * V; j < (k + 1) * V; j += 4)
+            *reinterpret_cast<float4 *>(out + P::first(k) + j - k * V) =
+                make_float4(s[j] * scale, s[j + 1] * scale, s[j + 2] * scale, s[j + 3] * scale);
+        }
       }
     } else {
       lds_barrier();
@@ -546,7 +607,7 @@ void step_bwd_rows_kernel(const StepArgs a) {
     const int64_t last = least(first + a.chunk_rows, (group + 1) * a.rows_per_gate);
     A.clear(a_lds);
     B.clear(b_lds);
-    load_branch<V, POST>(a, group, pl.c, pl.n, kp);
+    load_branch<POST>(a, group, pl, kp);
     auto ask_pre = [&](Row &r, int64_t base) {
       const uint32_t rows = rows_in<RPB>(base, last);
       const int64_t off = base * a.cols * static_cast<int64_t>(sizeof(T));
@@ -584,18 +645,18 @@ void step_bwd_rows_kernel(const StepArgs a) {
       const uint32_t rows = rows_in<RPB>(base, last);
       const int64_t off = base * a.cols * static_cast<int64_t>(sizeof(T));
       const bool in = RPB == 1 || pl.stat < 4 * rows;
-      float t[V];
+      float t[W];
       if constexpr (PRE) {
         const float rho = in ? inv_std(r.v2, a.eps) : 0.f, mu = r.m2;
-        float s[S], hh[V], d[V];
+        float s[S], hh[W], d[W];
 #pragma unroll
         for (int i = 0; i < S; ++i) s[i] = 0.f;
         r.h.template unit<LN>(a, mu, rho, hh);
-        Tok<T>::unpack(r.dy, d);
+        P::unpack(r.dy, d);
         C.load(c_lds);
         if constexpr (LN) E.load(e_lds);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
+        for (int j = 0; j < W; ++j) {
           C.add(c_lds, j, d[j], hh[j]);
           if constexpr (LN) E.add(e_lds, j, d[j], 1.f);
           d[j] *= gn[j];
@@ -605,31 +666,30 @@ void step_bwd_rows_kernel(const StepArgs a) {
         C.save(c_lds);
         if constexpr (LN) E.save(e_lds);
         r.h.pin();
-        if constexpr (sizeof(T) == 2)
-          asm volatile("" : "+v"(r.dy.v.x), "+v"(r.dy.v.y), "+v"(r.dy.v.z), "+v"(r.dy.v.w));
+        r.dy.pin();
         row_total<TPR, S>(s, lds, turn);
         const float s2 = s[0] * inv, s1 = LN ? s[S - 1] * inv : 0.f;
         r.h.template unit<LN>(a, mu, rho, hh);
-        Tok<T>::unpack(r.dy, d);
-        Tok<T>::unpack(r.dh, t);
+        P::unpack(r.dy, d);
+        P::unpack(r.dh, t);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
+        for (int j = 0; j < W; ++j) {
           t[j] = fmaf(rho, fmaf(d[j], gn[j], -(LN ? fmaf(hh[j], s2, s1) : hh[j] * s2)), t[j]);
         }
       } else {
-        Tok<T>::unpack(r.dh, t);
+        P::unpack(r.dh, t);
       }
       settle(t);
       ask_pre(r, base + D * RPB);
       {
-        float o[V];
+        float o[W];
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = a.res_scale * t[j];
+        for (int j = 0; j < W; ++j) o[j] = a.res_scale * t[j];
         pl.put(buffer(a.dres, off, rows * row_bytes),
                buffer(a.accum & NBLAHIP_ACCUM_DRES ? a.dres : nullptr, off, rows * row_bytes), o);
       }
       const float rho = POST ? in ? inv_std(r.v1, a.eps) : 0.f : 1.f, mu = POST ? r.m1 : 0.f;
-      float m[S], xh[V];
+      float m[S], xh[W];
 #pragma unroll
       for (int i = 0; i < S; ++i) m[i] = 0.f;
       if constexpr (POST)
@@ -638,22 +698,22 @@ void step_bwd_rows_kernel(const StepArgs a) {
         r.x.get(a, xh);
       if constexpr (OPTIONS) {
         const bool full = a.gate_kind == 2;
-        float g[V];
-        if constexpr (POST && LN) load_bias<V>(full ? a.beta_post : nullptr, pl.c, pl.n, g);
+        float g[W];
+        if constexpr (POST && LN) pl.bias(full ? a.beta_post : nullptr, g);
 #pragma unroll
-        for (int j = 0; j < V; ++j)
+        for (int j = 0; j < W; ++j)
           g[j] = t[j] * (POST && LN ? fmaf(xh[j], kp[j], a.branch_scale * g[j]) : xh[j] * kp[j]);
         pl.put(buffer(full ? a.dgate : nullptr, off, rows * row_bytes),
                buffer(full && (a.accum & NBLAHIP_ACCUM_DGATE) ? a.dgate : nullptr, off, rows * row_bytes), g);
-        Tok<T>::unpack(r.gf, g);
+        P::unpack(r.gf, g);
 #pragma unroll
-        for (int j = 0; j < V; ++j) t[j] *= full ? g[j] : 1.f;
+        for (int j = 0; j < W; ++j) t[j] *= full ? g[j] : 1.f;
       }
       // branch_scale and a shared gate are multiplied in after the column sums
       A.load(a_lds);
       if constexpr (LN && POST) B.load(b_lds);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
+      for (int j = 0; j < W; ++j) {
         A.add(a_lds, j, t[j], xh[j]);
         if constexpr (LN && POST) B.add(b_lds, j, t[j], 1.f);
         t[j] *= kp[j];
@@ -672,7 +732,7 @@ void step_bwd_rows_kernel(const StepArgs a) {
         const float s2 = m[0] * inv, s1 = LN ? m[S - 1] * inv : 0.f;
         if constexpr (PRE) r.x.template unit<LN>(a, mu, rho, xh);
 #pragma unroll
-        for (int j = 0; j < V; ++j)
+        for (int j = 0; j < W; ++j)
           t[j] = rho * (t[j] - (LN ? fmaf(xh[j], s2, s1) : xh[j] * s2));
       }
       settle(t);
@@ -683,7 +743,7 @@ void step_bwd_rows_kernel(const StepArgs a) {
     }
     if (a.part_post) {
       float *out = a.part_post + chunk * S * a.pitch;
-      float s[V];
+      float s[W];
       A.get(a_lds, s);
       flush(out, s, a.branch_scale);
       if constexpr (LN) {
@@ -694,7 +754,7 @@ void step_bwd_rows_kernel(const StepArgs a) {
   }
   if (PRE && a.part_pre) {
     float *out = a.part_pre + static_cast<int64_t>(blockIdx.x) * S * a.pitch;
-    float s[V];
+    float s[W];
     C.get(c_lds, s);
     flush(out, s, 1.f);
     if constexpr (LN) {

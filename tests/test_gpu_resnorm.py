@@ -88,6 +88,19 @@ def test_blocks_of_1024_threads(post, pre, norm, dtype, kept):
         run(Step(18, cols, dtype, norm, post, pre, True, gate, samples=3), kept)
 
 
+@pytest.mark.parametrize("kept", [None, "int8", "e4m3"])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize("post,pre", [(True, True), (True, False), (False, True)])
+def test_two_vectors_per_thread(post, pre, norm, dtype, kept):
+    """Rows of more vectors than a block has threads: in registers where they fit,
+    else through the kernels for long rows; whole, ragged, a gate per element."""
+    wide = 1 if dtype == "f32" else 2
+    for cols, gate in ((8192 * wide, "sample"), (4096 * wide + 4 * wide, "channel"),
+                       (5001 * wide + 1, "none"), (6000 * wide, "full")):
+        run(Step(10, cols, dtype, norm, post, pre, True, gate, samples=2), kept)
+
+
 @pytest.mark.parametrize("norm", ["rms", "layer"])
 def test_without_parameters(norm):
     run(Step(40, 520, "f16", norm, gate="sample", samples=4, affine=False))
