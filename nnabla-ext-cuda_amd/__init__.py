@@ -646,25 +646,34 @@ def _one_gpu(first, *rest):
     index = first.get_device()
     if index < 0:
         raise TypeError(f"tensors must be on a GPU, not on {first.device}")
-    if not first.is_contiguous():
-        raise ValueError("tensors must be contiguous")
+    ok = first.is_contiguous()
     for t in rest:
         if t is not None:
             if t.get_device() != index:
                 raise ValueError(f"tensors on {first.device} and on {t.device} in one call")
-            if not t.is_contiguous():
-                raise ValueError("tensors must be contiguous")
+            ok = ok and t.is_contiguous()
+    if not ok:
+        raise ValueError("tensors must be contiguous")
     return index
+
+
+def _stream_of(index):
+    """GPU `index`'s current stream, and what to hold while launching on it (None
+    where it is the current device)."""
+    import torch
+    if index == torch.cuda.current_device():
+        return torch._C._cuda_getCurrentRawStream(index), None
+    return torch._C._cuda_getCurrentRawStream(index), torch.cuda.device(index)
 
 
 def _call(index, fn, *args):
     """fn(*args, stream) on GPU `index`, on that GPU's current stream."""
-    import torch
-    if index == torch.cuda.current_device():
-        code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    stream, device = _stream_of(index)
+    if device is None:
+        code = fn(*args, stream)
     else:
-        with torch.cuda.device(index):
-            code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        with device:
+            code = fn(*args, stream)
     if code != 0:
         check(code)
 
@@ -891,36 +900,41 @@ def resnorm_backward(x, h, dh, dy, stats, outer, gate=None, gamma_post=None, bet
     hd, hs, hf = _check_kept(h, "h", rows, cols, act)
     if x is not None and h is not None and xf != hf:
         raise TypeError("x and h must be kept in the same form")
-    out = (None,) * 7 if out is None else out
+    given = out if out is not None else (None,) * 7
     gpu = _one_gpu(lead, dh, dy, xd, xs, hd, hs, gate, gamma_post, beta_post, gamma_pre, beta_pre,
-                   *stats, *out, ws)
+                   *stats, *given, ws)
     _step_params(cols, post, pre, kind, gamma_post, beta_post, gamma_pre, beta_pre)
-    _like(dh, rows * cols, act, "dh")
-    _like(dy, rows * cols, act, "dy")
+    n = rows * cols
+    _like(dh, n, act, "dh")
+    _like(dy, n, act, "dy")
     for s, name in zip(stats, ("mean_post", "var_post", "mean_pre", "var_pre")):
         _like(s, rows, torch.float32, name)
     dev, f32 = lead.device, torch.float32
-    shape, par = (lead.shape, rows * cols, act), ((cols,), cols, f32)
-    shapes = (shape, shape,
-              None if gate is None else (gate.shape, gate.numel(), act if gk == 2 else f32),
-              par, par, par, par)
-    have = (True, has_res, gk != 0, post, post and layer, pre, pre and layer)
-    grads, mask = [], 0
-    for i in range(7):
-        t = None
-        if have[i] and need[i]:
-            t = out[i]
-            if t is None:
-                t = torch.empty(shapes[i][0], dtype=shapes[i][2], device=dev)
-            else:
-                _like(t, shapes[i][1], shapes[i][2], ResNormGrads._fields[i])
-            if accum[i]:
+
+    def tensor(i):
+        t = given[i]
+        return torch.empty_like(lead) if t is None else _like(t, n, act, ResNormGrads._fields[i])
+
+    def param(i):
+        t = given[i]
+        return torch.empty(cols, dtype=f32, device=dev) if t is None else _like(
+            t, cols, f32, ResNormGrads._fields[i])
+    dgate = None
+    if gk and need[2]:
+        dgate = torch.empty_like(gate) if given[2] is None else _like(
+            given[2], gate.numel(), gate.dtype, "dgate")
+    grads = (tensor(0) if need[0] else None, tensor(1) if has_res and need[1] else None, dgate,
+             param(3) if post and need[3] else None, param(4) if post and layer and need[4] else None,
+             param(5) if pre and need[5] else None, param(6) if pre and layer and need[6] else None)
+    mask = 0
+    if any(accum):
+        for i in range(7):
+            if accum[i] and grads[i] is not None:
                 mask |= _ACCUM_BITS[i]
-        grads.append(t)
     if ws is None:
         ws = _workspace(lib().nblahip_resnorm_bwd_workspace_bytes(
             rows, cols, gk, gr, kind, int(post), int(pre), dt), dev)
-    p = [_ptr(g) for g in grads]
+    p = [None if g is None else g.data_ptr() for g in grads]
     _call(gpu, lib().nblahip_resnorm_bwd, _ptr(xd), _ptr(xs), _ptr(hd), _ptr(hs), xf or hf, _ptr(dh),
           _ptr(dy), _ptr(gate), gk, gr, _ptr(gamma_post), _ptr(beta_post), _ptr(gamma_pre),
           _ptr(stats[0]), _ptr(stats[1]), _ptr(stats[2]), _ptr(stats[3]), p[0], p[1], p[2], p[3], p[4],
