@@ -424,17 +424,21 @@ NBLAHIP_EXPORT int nblahip_in_cl_bwd(const void *x, const void *dy,
  *
  * Tensors are [rows, cols], contiguous, a row per token; dtype is NBLAHIP_F32,
  * NBLAHIP_F16 or NBLAHIP_BF16.  Any number of rows and columns (cols below
- * 2^31, fewer than 2^46 elements) at element alignment.  Parameters, shared
+ * 2^27, fewer than 2^46 elements; more: NBLAHIP_ERANGE) at element alignment.  Parameters, shared
  * gates, statistics and their gradients are float32, all arithmetic too; each
  * output is rounded once.  The norms are over the columns:
  *   RMS   : v / sqrt(mean(v^2) + eps) * gamma               (saved: mean square)
  *   LAYER : (v - mean) / sqrt(var + eps) * gamma + beta     (saved: mean, biased var)
- * A NULL gamma / beta stands for 1 / 0; RMS has no beta.
+ * A NULL gamma / beta stands for 1 / 0; RMS has no beta.  A row whose sum, sum of
+ * squares or mean / std leaves float32's range, or that holds an infinity or NaN,
+ * has infinities or NaN in its outputs; other rows' outputs do not.
  *
  * Aliasing: an output tensor may be an input tensor of its shape and dtype
  * itself (h may be res: the stream is updated in place); other overlaps of an
  * output with an input, a parameter, a saved statistic, the workspace or
- * another output are refused with NBLAHIP_EALIAS.
+ * another output are refused with NBLAHIP_EALIAS.  A workspace serves one call
+ * at a time (calls, or replays of captured ones, that may run at once need one
+ * each).
  * ---------------------------------------------------------------------- */
 
 /* 8-bit copies of activations.  Each run of 32 columns of a row (the last may
@@ -443,7 +447,9 @@ NBLAHIP_EXPORT int nblahip_in_cl_bwd(const void *x, const void *dy,
  * less (INT8: two's complement), is 448 or less (E4M3: 4 exponent and 3
  * mantissa bits, finite only).  Codes are rounded to nearest, ties to even.  A
  * run that holds an infinity or NaN has code 255 and reads back as NaN.  A copy
- * of rows x cols is rows*cols bytes of codes and rows*ceil(cols/32) of scales. */
+ * of rows x cols is rows*cols bytes of codes and rows*ceil(cols/32) of scales.
+ * Pack and unpack take copies of fewer than 2^34 16-byte vectors of x, each row
+ * counted up to whole runs. */
 enum nblahip_act8_format { NBLAHIP_ACT8_NONE = 0, NBLAHIP_ACT8_INT8 = 1, NBLAHIP_ACT8_E4M3 = 2 };
 
 NBLAHIP_EXPORT int64_t nblahip_act8_scales_per_row(int64_t cols);
@@ -496,8 +502,9 @@ NBLAHIP_EXPORT int nblahip_ln_bwd_act8(const void *x8, const uint8_t *x_scale,
  * gate_kind: NONE; ROWS: float32 [gate_rows, cols], gate row g scales rows
  * g*rows/gate_rows onward (1: a learned scale per channel; a row per sample: the
  * gate of a conditioned block), gate_rows divides rows; FULL: [rows, cols] of
- * dtype.  x8 / h8 with their scales (each pair may be NULL) receive the 8-bit
- * copies of x and of h as stored that nblahip_act8_pack would make. */
+ * dtype.  x8 / h8 with their scales (each pair may be NULL; h8 with pre only)
+ * receive the 8-bit copies of x and of h as stored that nblahip_act8_pack would
+ * make. */
 enum nblahip_norm_kind { NBLAHIP_NORM_RMS = 0, NBLAHIP_NORM_LAYER = 1 };
 enum nblahip_gate_kind { NBLAHIP_GATE_NONE = 0, NBLAHIP_GATE_ROWS = 1, NBLAHIP_GATE_FULL = 2 };
 

@@ -693,6 +693,11 @@ def _like(t, n, dtype, name):
     return t
 
 
+def _check_adds(adds, name, given):
+    if adds and given is None:
+        raise ValueError(f"{name}: accumulation needs the tensor to add to")
+
+
 def _check_kept(k, name, rows, cols, dtype):
     """A kept tensor (or its 8-bit copy) of rows x cols: (data, scales, format)."""
     import torch
@@ -761,6 +766,8 @@ def rms_backward(x, dy, gamma, ms, outer, eps=1e-5, dx=None, dgamma=None, accum=
     gpu = _one_gpu(dy, xd, xs, gamma, ms, dx, dgamma, ws)
     _like(gamma, cols, torch.float32, "gamma")
     _like(ms, rows, torch.float32, "ms")
+    _check_adds(need[0] and accum[0], "dx", dx)
+    _check_adds(need[1] and accum[1], "dgamma", dgamma)
     dx = None if not need[0] else torch.empty_like(dy) if dx is None else _like(
         dx, rows * cols, dy.dtype, "dx")
     dgamma = None if not need[1] else torch.empty(
@@ -786,6 +793,8 @@ def ln_backward_act8(x8, dy, gamma, mean, var, outer, eps=1e-5, dx=None, dgamma=
     _like(gamma, cols, torch.float32, "gamma")
     _like(mean, rows, torch.float32, "mean")
     _like(var, rows, torch.float32, "var")
+    for i, t, name in ((0, dx, "dx"), (1, dgamma, "dgamma"), (2, dbeta, "dbeta")):
+        _check_adds(need[i] and accum[i], name, t)
     dx = None if not need[0] else torch.empty_like(dy) if dx is None else _like(
         dx, rows * cols, dy.dtype, "dx")
     par = [None if not need[i] else torch.empty(cols, dtype=torch.float32, device=dy.device)
@@ -930,6 +939,7 @@ def resnorm_backward(x, h, dh, dy, stats, outer, gate=None, gamma_post=None, bet
     if any(accum):
         for i in range(7):
             if accum[i] and grads[i] is not None:
+                _check_adds(True, ResNormGrads._fields[i], given[i])
                 mask |= _ACCUM_BITS[i]
     if ws is None:
         ws = _workspace(lib().nblahip_resnorm_bwd_workspace_bytes(

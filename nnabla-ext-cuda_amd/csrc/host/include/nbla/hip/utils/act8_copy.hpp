@@ -60,8 +60,8 @@ inline void rows_and_columns(const string &name, const Shape_t &shape, vector<in
   }
   cols = 1;
   for (size_t i = batch_axis.size(); i < shape.size(); ++i) cols *= shape[i];
-  NBLA_CHECK(cols < (Size_t(1) << 31), error_code::value,
-             "%s: fewer than 2^31 elements per row required.", name.c_str());
+  NBLA_CHECK(cols < (Size_t(1) << 27), error_code::value,
+             "%s: fewer than 2^27 elements per row required.", name.c_str());
 }
 
 } // namespace nbla

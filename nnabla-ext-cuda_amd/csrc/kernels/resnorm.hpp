@@ -41,7 +41,7 @@ struct StepArgs {
   int64_t groups8 = 0;           // 8-bit groups per row
   int gate_kind = 0;
   int format8 = 0;
-  int grid = 1;                  // blocks launched (= rows of part_pre)
+  int64_t grid = 1;              // row kernels: blocks launched; backward: rows of part_pre
   float res_scale = 1.f, branch_scale = 1.f, eps = 0.f;
 };
 

@@ -11,7 +11,7 @@ using namespace nblahip;
 
 namespace {
 
-constexpr int64_t kMaxCols = (1ll << 31) - 1;
+constexpr int64_t kMaxCols = (1ll << 27) - 1; // the fold's grid: 16 threads per column, fewer than 2^32
 constexpr int64_t kGridY = 65535;
 
 hipStream_t as_stream(void *s) { return static_cast<hipStream_t>(s); }
@@ -117,12 +117,12 @@ size_t plan_bwd(StepArgs &a, StepPlan &pl, int64_t gate_rows, char *ws) {
   a.pitch = (a.cols + 7) / 8 * 8;
   if (pl.tpr == 0) {
     plan_chunks(a, gate_rows, kCus, 16);
-    a.grid = static_cast<int>(std::min<int64_t>(a.chunks, 1 << 30));
+    a.grid = a.chunks;
   } else {
     const int block = bwd_block(pl.tpr);
     const int64_t blocks = kCus * bwd_blocks_per_cu(vec_of(pl.dtype), pl.layer, pl.post, pl.pre, pl.kept8, pl.mode, pl.tpr);
     plan_chunks(a, gate_rows, blocks, block / pl.tpr);
-    a.grid = static_cast<int>(std::min<int64_t>(a.chunks, blocks));
+    a.grid = std::min<int64_t>(a.chunks, blocks);
   }
   size_t at = 0;
   auto take = [&](int64_t floats) {
@@ -289,6 +289,8 @@ int step_fwd(StepArgs a, StepPlan pl, int64_t gate_rows, hipStream_t st) {
   if ((a.x8 == nullptr) != (a.x8_scale == nullptr) || (a.h8 == nullptr) != (a.h8_scale == nullptr))
     return NBLAHIP_EINVAL;
   if ((a.x8 || a.h8) && !format_ok(a.format8)) return NBLAHIP_EINVAL;
+  if (a.h8 && !pl.pre) return NBLAHIP_EINVAL; // (the backward reads h for the second norm alone)
+  if (!a.res) a.res_scale = 0.f;              // (an infinite one must not meet the zeros read for res)
   const size_t n = static_cast<size_t>(a.rows) * a.cols, tb = n * elem_bytes(pl.dtype);
   const size_t pb = 4 * static_cast<size_t>(a.cols), sb = 4 * static_cast<size_t>(a.rows);
   a.groups8 = groups_of(a.cols);
@@ -316,7 +318,7 @@ int step_fwd(StepArgs a, StepPlan pl, int64_t gate_rows, hipStream_t st) {
   const int block = pl.tpr ? fwd_block(pl.tpr) : 1024;
   const int64_t blocks = kCus * (2048 / block);
   plan_chunks(a, gate_rows, blocks, pl.tpr ? block / pl.tpr : 1);
-  a.grid = static_cast<int>(std::min<int64_t>(a.chunks, blocks));
+  a.grid = std::min<int64_t>(a.chunks, blocks);
   return run_fwd(pl, a, st);
 }
 

@@ -173,6 +173,31 @@ def test_gradients_that_are_not_needed_and_accumulation(cols):
         assert ((a - (b + c)).abs() <= 2.0 ** -22 * (b.abs() + c.abs())).all(), n
 
 
+def test_accumulation_needs_a_tensor_to_add_to():
+    st = Step(6, 64, "f16", "layer", gate="sample", samples=2)
+    f, g = run(st)
+    for i, name in enumerate(g._fields):
+        with pytest.raises(ValueError, match=name):
+            K.resnorm_backward(st.x, f.h, st.dh, st.dy, f.stats, 6, accum=[k == i for k in range(7)],
+                               **st.args())
+    x8 = K.act8_pack(st.x, 6)
+    for i, name in enumerate(("dx", "dgamma", "dbeta")):
+        accum = [k == i for k in range(3)]
+        with pytest.raises(ValueError, match=name):
+            K.ln_backward_act8(x8, st.dy, None, f.stats[0], f.stats[1], 6, accum=accum)
+        if i < 2:
+            with pytest.raises(ValueError, match=name):
+                K.rms_backward(st.x, st.dy, None, f.stats[1], 6, accum=accum[:2])
+
+
+@pytest.mark.parametrize("cols", [520, 1030, 33000])
+def test_scale_of_an_absent_residual_is_not_read(cols):
+    x = torch.randn(3, cols, device="cuda")
+    want = K.resnorm_forward(x, None, 3)
+    got = K.resnorm_forward(x, None, 3, res_scale=float("inf"))
+    assert torch.equal(got.h, want.h) and torch.equal(got.y, want.y)
+
+
 def test_in_place():
     for cols in (520, 1030, 33000):
         st = Step(20, cols, "f16", "layer", gate="full")

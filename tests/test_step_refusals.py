@@ -57,8 +57,9 @@ def bwd_args(**over):
     (dict(gate=BASE, gate_kind=4, gate_rows=1), EINVAL),
     (dict(x8=BASE, f=1), EINVAL), (dict(x8=BASE, x8s=BASE + 65536, f=0), EINVAL),
     (dict(h8=BASE, h8s=BASE + 65536, f=3), EINVAL),
-    (dict(rows=-1), EINVAL), (dict(cols=-1), EINVAL), (dict(cols=1 << 31), ERANGE),
+    (dict(rows=-1), EINVAL), (dict(cols=-1), EINVAL), (dict(cols=1 << 27), ERANGE),
     (dict(rows=1 << 40, cols=1 << 20), ERANGE),
+    (dict(post=1, pre=0, gn=None, h8=BASE, h8s=BASE + 65536, f=1), EINVAL),
     (dict(rows=0), 0), (dict(cols=0), 0),
 ])
 def test_forward_refusals(over, code):
@@ -86,7 +87,7 @@ def test_forward_overlaps():
     (dict(gate=BASE, gate_kind=1, gate_rows=5), EINVAL), (dict(gate=BASE, gate_kind=2, gate_rows=0,
                                                                dgate=BASE + 2), EALIAS),
     (dict(ws=None), EWORKSPACE), (dict(wsn=16), EWORKSPACE), (dict(ws=BASE + 128), EWORKSPACE),
-    (dict(rows=-3), EINVAL), (dict(cols=1 << 31), ERANGE), (dict(cols=0), 0),
+    (dict(rows=-3), EINVAL), (dict(cols=1 << 27), ERANGE), (dict(cols=0), 0),
 ])
 def test_backward_refusals(over, code):
     assert L.nblahip_resnorm_bwd(*bwd_args(**over)) == code
@@ -130,7 +131,7 @@ def test_act8_refusals():
         a = (x, q, s) if f is L.nblahip_act8_pack else (q, s, x)
         assert f(*a, 4, 64, 0, 1, None) == EINVAL and f(*a, 4, 64, 1, 3, None) == EINVAL
         assert f(None, *a[1:], 4, 64, 1, 1, None) == EINVAL and f(*a[:2], None, 4, 64, 1, 1, None) == EINVAL
-        assert f(*a, -1, 64, 1, 1, None) == EINVAL and f(*a, 4, 1 << 31, 1, 1, None) == ERANGE
+        assert f(*a, -1, 64, 1, 1, None) == EINVAL and f(*a, 4, 1 << 27, 1, 1, None) == ERANGE
         assert f(*a, 0, 64, 1, 1, None) == 0
     assert L.nblahip_act8_pack(x, x + 100, s, 4, 64, 1, 1, None) == EALIAS
     assert L.nblahip_act8_pack(x, q, q + 255, 4, 64, 1, 1, None) == EALIAS
@@ -155,6 +156,12 @@ def test_workspace_sizes():
         for g, n in ((0, 0), (1, 1), (2, 0)):
             b = w(rows, cols, g, n, 1, 1, 1, 2)
             assert b % 256 == 0 and 0 < b < 64 * rows * cols + (1 << 20)
+
+
+def test_workspace_holds_a_partial_sum_per_gate_row():
+    # one column, a gate row per row: a partial row (8 floats) per gate row
+    n = (1 << 30) + 4096
+    assert L.nblahip_resnorm_bwd_workspace_bytes(n, 1, 1, n, 0, 0, 1, 1) >= n * 32 * 2 + n * 16
 
 
 def test_wrappers_refuse():
