@@ -53,6 +53,10 @@ template <> __device__ __forceinline__ float widen16<bf16>(uint32_t w, bool high
 // Two floats rounded to nearest even and packed (one instruction each on gfx950).
 template <typename T> __device__ __forceinline__ uint32_t narrow16(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t narrow16<__half>(float lo, float hi) {
+  // (The compiler would round a product and sum to float16 at once, by a mixed-
+  // precision instruction: another value than that of the float32 result, which it
+  // computes beside it where that is needed too.)
+  asm("" : "+v"(lo), "+v"(hi));
   const half2_native h = {static_cast<_Float16>(lo), static_cast<_Float16>(hi)};
   return __builtin_bit_cast(uint32_t, h);
 }
