@@ -61,7 +61,7 @@ struct StepPlan {
 // vectors per thread.
 #define NBLAHIP_STEP_LAYOUTS(CASE)                                                            \
   CASE(16, 1) CASE(32, 1) CASE(64, 1) CASE(128, 1) CASE(192, 1) CASE(256, 1) CASE(384, 1)     \
-  CASE(512, 1) CASE(640, 1) CASE(768, 1) CASE(1024, 1) CASE(1024, 2)
+  CASE(512, 1) CASE(640, 1) CASE(768, 1) CASE(1024, 1) CASE(1024, 2) CASE(512, 4)
 
 // Threads of a block.  Backward: 512 where a row takes 256 or fewer, so that the
 // rows of a block share one partial sum per column (half the partial sums of
@@ -80,7 +80,8 @@ constexpr int bwd_waves(int vec, bool layer, bool post, bool pre, bool q8, int m
   if (layer) return (pre ? 4 : 5) - (mode != kWhole ? 1 : 0);
   return mode == kWhole ? (pre ? 5 : 6) : mode == kRagged && !(both && q8) ? 5 : 4;
 }
-constexpr int bwd_blocks_per_cu(int vec, bool layer, bool post, bool pre, bool q8, int mode, int tpr) {
+constexpr int bwd_blocks_per_cu(int vec, bool layer, bool post, bool pre, bool q8, int mode, int tpr, int nv) {
+  if (nv == 4) return 1;
   const int n = 256 * bwd_waves(vec, layer, post, pre, q8, mode, tpr) / bwd_block(tpr);
   return n > 0 ? n : 1;
 }
@@ -91,36 +92,47 @@ constexpr int bwd_blocks_per_cu(int vec, bool layer, bool post, bool pre, bool q
 constexpr int bwd_depth(int vec, bool layer, bool post, bool pre, bool q8, int mode, int tpr, int nv) {
   if (nv > 1) return 1;
   const bool full = tpr == 1024 && (vec == 8 ? mode != kWhole || (layer && post && pre) : mode != kWhole && layer);
-  const int blocks = bwd_blocks_per_cu(vec, layer, post, pre, q8, mode, tpr);
+  const int blocks = bwd_blocks_per_cu(vec, layer, post, pre, q8, mode, tpr, nv);
   return (blocks == 1 && !full) || (blocks == 2 && vec == 8 && !layer && mode == kWhole && tpr == 512) ? 2 : 1;
 }
+// Forward the same for blocks of 256 threads and more.
 constexpr int fwd_depth(int tpr, int nv, int mode) {
   return tpr >= 256 && nv == 1 && !(mode != kWhole && tpr == 1024) ? 2 : 1;
 }
 // Column sums (C, A: of gradient times normalized value; E, B: of the gradient; C
-// and E of the second norm) that a block of 1024 threads keeps in LDS, at most
-// 128 KB, because its 128 registers a thread are taken.  w: columns of a
-// thread.
+// and E of the second norm) that a block keeps in LDS, at most 128 KB, because its
+// registers are taken: 128 a thread of a block of 1024, 256 where threads have four
+// vectors.  w: columns of a thread.
 enum { kSumC = 1, kSumE = 2, kSumA = 4, kSumB = 8 };
 constexpr unsigned bwd_sums_in_lds(int w, bool layer, bool post, bool pre, bool q8, int mode, int tpr) {
+  if (w == 32) return layer ? (pre ? kSumC | kSumE : kSumA | kSumB) : (pre ? kSumC : 0) | kSumA;
   if (tpr != 1024 || w < 8) return 0;
   if (w == 8)
     return (layer ? kSumE | kSumB : 0) | (mode != kWhole || (layer && q8) ? kSumA : 0) |
            (layer && (mode != kWhole || q8) ? kSumC : 0);
   return kSumA; // (of 16 columns: the RMS norm alone, see bwd_row_fits)
 }
-// Forms that do not fit the registers (and LDS) of a block of 1024: they run as
-// long rows.
+// Which forms the layouts of the longest rows have: what fits their registers and
+// LDS.  1024 threads of two vectors come first, 512 of four are for forms that do
+// not fit those (as fast where both fit, slower for ragged rows: [2048, 8191] float
+// pre-norm backward 111 us in twos, 143 in fours); what fits neither runs as long
+// rows.  [2048, 16384] bf16 RMS step backward: long 183 us, fours 101.
 constexpr bool bwd_row_fits(int vec, bool layer, bool post, bool pre, bool q8, int mode, int tpr, int nv) {
-  if (tpr < 1024) return true;
-  if (nv == 1) return !(vec == 8 && layer && post && pre && mode != kWhole);
-  if (vec == 8) return mode == kWhole && post && !pre && !layer;
-  return mode == kWhole ? !(layer && post && pre) : !(post && pre) && !(layer && pre && q8);
+  const bool both = post && pre;
+  if (tpr < 1024 && nv == 1) return true;
+  if (nv == 1) return !(vec == 8 && layer && both && mode != kWhole);
+  const bool twos = vec == 8         ? mode == kWhole && post && !pre && !layer
+                    : mode == kWhole ? !(layer && both)
+                                     : !both && !(layer && pre && q8);
+  if (nv == 2) return twos;
+  return !twos && (vec == 8 ? mode == kWhole && !(layer && both) : mode == kWhole || (!layer && !q8));
 }
 constexpr bool fwd_row_fits(int vec, bool layer, bool post, bool pre, bool copy, int mode, int nv) {
   if (nv == 1) return true;
-  if (vec == 4) return !(layer && post && mode != kWhole);
-  return mode == kWhole && !(layer && post) && !(copy && pre);
+  const bool twos = vec == 8 ? mode == kWhole && !(layer && post) && !(copy && pre)
+                             : !(layer && post && mode != kWhole);
+  if (nv == 2) return twos;
+  return !twos && (vec == 8 ? mode == kWhole && !(layer && post && pre && copy) : !(pre && copy));
 }
 
 int launch_step_fwd_f32(const StepPlan &pl, const StepArgs &a, hipStream_t st);

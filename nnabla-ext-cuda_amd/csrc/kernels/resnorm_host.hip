@@ -64,20 +64,23 @@ constexpr int kCus = 256;
 
 int vec_of(int dtype) { return dtype == NBLAHIP_F32 ? 4 : 8; }
 
-// The layout with just enough threads for the row's vectors; rows longer than any
-// of them, and those of less than a vector, go to the kernels for long rows.
-void pick_layout(StepPlan &pl, int64_t cols) {
+// The layout with just enough threads for the row's vectors, of those that have the
+// form (fits); rows longer than any of them, and those of less than a vector, go to
+// the kernels for long rows.
+template <typename F> void pick_layout(StepPlan &pl, int64_t cols, F fits) {
   const int64_t vec = vec_of(pl.dtype), vectors = (cols + vec - 1) / vec;
   pl.tpr = pl.nv = 0;
   if (cols < vec) return;
-#define NBLAHIP_CASE(TPR, NV)             \
-  if (pl.tpr == 0 && vectors <= TPR * NV) { \
-    pl.tpr = TPR;                         \
-    pl.nv = NV;                           \
+  int mode = pl.mode;
+#define NBLAHIP_CASE(TPR, NV)                                                \
+  if (NV > 1 && mode == kRagged) mode = kAny; /* (one form for both) */      \
+  if (pl.tpr == 0 && vectors <= TPR * NV && fits(mode, TPR, NV)) {           \
+    pl.mode = mode;                                                          \
+    pl.tpr = TPR;                                                            \
+    pl.nv = NV;                                                              \
   }
   NBLAHIP_STEP_LAYOUTS(NBLAHIP_CASE)
 #undef NBLAHIP_CASE
-  if (pl.nv > 1 && pl.mode == kRagged) pl.mode = kAny; // (one form for both)
 }
 
 // Whether every address that a 16-byte vector of the tensors (or its 8-bit
@@ -111,16 +114,16 @@ int64_t shared_gate_rows(const StepArgs &a, int64_t gate_rows) {
 
 // The backward's split, and its workspace laid out from `ws` (null: sizes only).
 size_t plan_bwd(StepArgs &a, StepPlan &pl, int64_t gate_rows, char *ws) {
-  pick_layout(pl, a.cols);
-  if (pl.tpr && !bwd_row_fits(vec_of(pl.dtype), pl.layer, pl.post, pl.pre, pl.kept8, pl.mode, pl.tpr, pl.nv))
-    pl.tpr = pl.nv = 0;
+  pick_layout(pl, a.cols, [&](int mode, int tpr, int nv) {
+    return bwd_row_fits(vec_of(pl.dtype), pl.layer, pl.post, pl.pre, pl.kept8, mode, tpr, nv);
+  });
   a.pitch = (a.cols + 7) / 8 * 8;
   if (pl.tpr == 0) {
     plan_chunks(a, gate_rows, kCus, 16);
     a.grid = a.chunks;
   } else {
     const int block = bwd_block(pl.tpr);
-    const int64_t blocks = kCus * bwd_blocks_per_cu(vec_of(pl.dtype), pl.layer, pl.post, pl.pre, pl.kept8, pl.mode, pl.tpr);
+    const int64_t blocks = kCus * bwd_blocks_per_cu(vec_of(pl.dtype), pl.layer, pl.post, pl.pre, pl.kept8, pl.mode, pl.tpr, pl.nv);
     plan_chunks(a, gate_rows, blocks, block / pl.tpr);
     a.grid = std::min<int64_t>(a.chunks, blocks);
   }
@@ -311,12 +314,12 @@ int step_fwd(StepArgs a, StepPlan pl, int64_t gate_rows, hipStream_t st) {
   pl.mode = a.gate_kind == NBLAHIP_GATE_FULL                                               ? kAny
             : whole_vectors(pl.dtype, a.cols, {a.x, a.res, a.h, a.y}, {a.x8, a.h8}) ? kWhole
                                                                                     : kRagged;
-  pick_layout(pl, a.cols);
-  if (pl.tpr && !fwd_row_fits(vec_of(pl.dtype), pl.layer, pl.post, pl.pre, a.x8 || a.h8, pl.mode, pl.nv))
-    pl.tpr = pl.nv = 0;
+  pick_layout(pl, a.cols, [&](int mode, int, int nv) {
+    return fwd_row_fits(vec_of(pl.dtype), pl.layer, pl.post, pl.pre, a.x8 || a.h8, mode, nv);
+  });
   gate_rows = shared_gate_rows(a, gate_rows);
   const int block = pl.tpr ? fwd_block(pl.tpr) : 1024;
-  const int64_t blocks = kCus * (2048 / block);
+  const int64_t blocks = kCus * (pl.nv == 4 ? 1 : 2048 / block); // (four vectors: 256 registers a thread)
   plan_chunks(a, gate_rows, blocks, pl.tpr ? block / pl.tpr : 1);
   a.grid = std::min<int64_t>(a.chunks, blocks);
   return run_fwd(pl, a, st);

@@ -5,10 +5,10 @@
 // bwd_row_fits and fwd_row_fits name.
 //
 // Bound by HBM and, on the way there, by reading twice: the forward's later
-// passes find the row in the caches ([2048, 12288] half LayerNormalization step
-// 80 us, 2.1 times its bytes' time), the backward's two kernels each read every
-// tensor ([2048, 16384] bf16 RMS step 182 us, 2.4 times; 75 for the row sums, 97
-// for the rest).
+// passes find the row in the caches ([2048, 16384] bf16 step of two
+// LayerNormalizations 119 us, 2.4 times its bytes' time), the backward's two
+// kernels each read every tensor (the same step 196 us, 2.6 times: 74 for the row
+// sums, 109 for the rest, 11 for the fold).
 #pragma once
 
 #include "resnorm.hpp"

@@ -1,12 +1,20 @@
-// The residual step on rows that fit a block at one or two 16-byte vectors per
-// thread: every tensor crosses HBM once per direction.
+// The residual step on rows that fit a block at one, two or four 16-byte vectors
+// per thread: every tensor crosses HBM once per direction.
 //
 // TPR threads hold a row; a block takes several rows at a time where they are
-// short.  A thread's columns are the same in every row, so the
-// parameters (and, backward, the column sums of the parameter gradients) stay
-// in its registers while the block walks its rows.
+// short.  A thread's columns are the same in every row, so the parameters (and,
+// backward, the column sums of the parameter gradients) stay in its registers
+// while the block walks its rows.  Row sums are float: a thread's columns, its
+// wave by DPP, waves through LDS.
 //
 // What bounds it: HBM (6 tensors of 2 bytes an element backward, 4 forward).
+// Forward [16384, 4096] bf16 RMS step 109 us, 4.9 TB/s of the 537 MB (a copy of
+// that size: 5.3); [16384, 1024] half LayerNormalization step 25 us, 5.4 TB/s.
+// Backward [8192, 8192] bf16 157 us + 5 of the fold, 5.1 TB/s; [16384, 1024] half
+// LayerNormalization 44 + 6 us, 4.6 TB/s; from 8 bits [8192, 4096] bf16 72 + 6 us,
+// 4.7 TB/s.  [2048, 16384] bf16 (four vectors) forward 56, backward 91 + 9 us.
+// Rows that end inside a vector take more instructions and requests: [8191, 4097]
+// bf16 backward 118 us, 3.4 TB/s, where whole rows of that size take 87.
 // A row's loads are asked for one row ahead and must stay in flight while the
 // row before is worked on and stored.  This GPU counts loads and stores in one
 // in-order counter per wave, and the compiler can wait for "all but the last
@@ -120,6 +128,12 @@ __device__ __forceinline__ uint4 shift_down_bits(uint4 v, uint32_t bits) {
 template <int N> __device__ __forceinline__ void settle(float (&v)[N]) {
 #pragma unroll
   for (int j = 0; j < N; ++j) asm volatile("" : "+v"(v[j]));
+}
+
+// Threads with four vectors work on them one after another: scheduled together
+// they take more registers than there are.
+template <int NV> __device__ __forceinline__ void one_vector_at_a_time() {
+  if constexpr (NV == 4) __builtin_amdgcn_sched_barrier(0);
 }
 
 // Where a thread's NV vectors lie in the rows a block has in hand, in bytes from
@@ -294,7 +308,7 @@ template <int RPB> __device__ __forceinline__ uint32_t rows_in(int64_t base, int
 
 // The second launch bound: waves per SIMD of the blocks a CU has at once.
 constexpr int bwd_bound(int vec, bool layer, bool post, bool pre, bool q8, int mode, int tpr, int nv) {
-  return (bwd_blocks_per_cu(vec, layer, post, pre, q8, mode, tpr) * bwd_block(tpr) + 255) / 256;
+  return (bwd_blocks_per_cu(vec, layer, post, pre, q8, mode, tpr, nv) * bwd_block(tpr) + 255) / 256;
 }
 
 // Forward.  A block takes runs of rows (chunks) that share a gate row.
@@ -312,8 +326,18 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
   const float inv = 1.f / static_cast<float>(a.cols);
   const uint32_t stat_out = threadIdx.x % TPR == 0 ? pl.stat : kOutside;
   float gn[W], bn[W], kp[W], kb[W];
+  // Two LayerNormalizations at four vectors: the second one's parameters wait in LDS.
+  constexpr bool PARK = LN && POST && PRE && W == 32;
+  __shared__ float4 park[PARK ? 2 * BLOCK * W / 4 : 1];
   if constexpr (PRE) pl.param(a.gamma_pre, gn);
   if constexpr (PRE && LN) pl.bias(a.beta_pre, bn);
+  if constexpr (PARK) {
+#pragma unroll
+    for (int j = 0; j < W / 4; ++j) {
+      park[(2 * j) * BLOCK + threadIdx.x] = make_float4(gn[4 * j], gn[4 * j + 1], gn[4 * j + 2], gn[4 * j + 3]);
+      park[(2 * j + 1) * BLOCK + threadIdx.x] = make_float4(bn[4 * j], bn[4 * j + 1], bn[4 * j + 2], bn[4 * j + 3]);
+    }
+  }
   for (int64_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
     const int64_t group = chunk / a.chunks_per_gate;
     const int64_t first = group * a.rows_per_gate + chunk % a.chunks_per_gate * a.chunk_rows;
@@ -413,9 +437,17 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
         const float rho2 = inv_std(v2, a.eps), shift2 = -m2 * rho2;
         float y[W];
 #pragma unroll
-        for (int j = 0; j < W; ++j)
+        for (int j = 0; j < W; ++j) {
+          if constexpr (PARK) {
+            if (j % 4 == 0) {
+              const float4 g = park[(j / 2) * BLOCK + threadIdx.x], b = park[(j / 2 + 1) * BLOCK + threadIdx.x];
+              gn[j] = g.x; gn[j + 1] = g.y; gn[j + 2] = g.z; gn[j + 3] = g.w;
+              bn[j] = b.x; bn[j + 1] = b.y; bn[j + 2] = b.z; bn[j + 3] = b.w;
+            }
+          }
           y[j] = !LN ? h[j] * rho2 * gn[j]
                      : fmaf(V == 8 ? fmaf(h[j], rho2, shift2) : (h[j] - m2) * rho2, gn[j], bn[j]);
+        }
         pl.store(buffer(a.y, off, bytes), P::pack(y));
       }
       if constexpr (POST) {
@@ -433,28 +465,30 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
 
 // A kept tensor's vectors as they were loaded: storage type, or an 8-bit copy.
 template <typename T, bool Q8, typename P> struct Kept {
-  static constexpr int W = P::W;
+  static constexpr int V = P::V;
   typename P::Vec p;
   __device__ __forceinline__ void ask(const StepArgs &a, const void *data, const uint8_t *, int64_t base,
                                       uint32_t rows, const P &pl) {
     p = pl.load(buffer(data, base * a.cols * static_cast<int64_t>(sizeof(T)),
                        rows * static_cast<uint32_t>(a.cols) * static_cast<uint32_t>(sizeof(T))));
   }
-  __device__ __forceinline__ void get(const StepArgs &, float (&o)[W]) const { P::unpack(p, o); }
+  __device__ __forceinline__ void get(const StepArgs &, int k, float (&o)[V]) const {
+    Tok<T>::unpack(p.p[k], o);
+  }
   // (value - mu) * rho.  16-bit data takes one fma, value * rho - mu * rho: off by
   // 2^-24 |mu| rho, far below what the data resolves; float data is centred first.
   template <bool CENTRED>
-  __device__ __forceinline__ void unit(const StepArgs &a, float mu, float rho, float (&o)[W]) const {
-    get(a, o);
+  __device__ __forceinline__ void unit(const StepArgs &a, float mu, float rho, int k, float (&o)[V]) const {
+    get(a, k, o);
     const float shift = -mu * rho;
 #pragma unroll
-    for (int j = 0; j < W; ++j)
+    for (int j = 0; j < V; ++j)
       o[j] = !CENTRED ? o[j] * rho : sizeof(T) == 2 ? fmaf(o[j], rho, shift) : (o[j] - mu) * rho;
   }
   __device__ __forceinline__ void pin() { p.pin(); }
 };
 template <typename T, typename P> struct Kept<T, true, P> {
-  static constexpr int W = P::W, V = P::V, NV = W / V;
+  static constexpr int V = P::V, NV = P::W / V;
   uint2 q[NV];
   uint32_t code[NV];
   __device__ __forceinline__ void ask(const StepArgs &a, const void *data, const uint8_t *scales,
@@ -467,22 +501,16 @@ template <typename T, typename P> struct Kept<T, true, P> {
       code[k] = __builtin_amdgcn_raw_buffer_load_b8(of, pl.scale[k], 0, 0);
     }
   }
-  __device__ __forceinline__ void get(const StepArgs &a, float (&o)[W]) const {
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-      act8_decode<V>(q[k], code[k], a.format8, reinterpret_cast<float(&)[V]>(o[k * V]));
+  __device__ __forceinline__ void get(const StepArgs &a, int k, float (&o)[V]) const {
+    act8_decode<V>(q[k], code[k], a.format8, o);
   }
   // One multiplication takes the scale (a power of two: exact) and rho.
   template <bool CENTRED>
-  __device__ __forceinline__ void unit(const StepArgs &a, float mu, float rho, float (&o)[W]) const {
-    const float shift = -mu * rho;
+  __device__ __forceinline__ void unit(const StepArgs &a, float mu, float rho, int k, float (&o)[V]) const {
+    const float shift = -mu * rho, scale = act8_scale(code[k]) * rho;
+    act8_numbers<V>(q[k], a.format8, o);
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const float scale = act8_scale(code[k]) * rho;
-      act8_numbers<V>(q[k], a.format8, reinterpret_cast<float(&)[V]>(o[k * V]));
-#pragma unroll
-      for (int j = k * V; j < (k + 1) * V; ++j) o[j] = CENTRED ? fmaf(o[j], scale, shift) : o[j] * scale;
-    }
+    for (int j = 0; j < V; ++j) o[j] = CENTRED ? fmaf(o[j], scale, shift) : o[j] * scale;
   }
   __device__ __forceinline__ void pin() {
 #pragma unroll
@@ -500,30 +528,32 @@ template <int W, int TPR, bool IN_LDS> struct ColumnSum {
     for (int j = 0; j < W; ++j) v[j] = 0.f;
   }
   __device__ __forceinline__ void add(float4 *, int j, float a, float b) { v[j] = fmaf(a, b, v[j]); }
-  __device__ __forceinline__ void load(float4 *) {}
-  __device__ __forceinline__ void save(float4 *) { settle(v); }
+  template <int V> __device__ __forceinline__ void load(float4 *, int) {}
+  template <int V> __device__ __forceinline__ void save(float4 *, int k) {
+    settle(reinterpret_cast<float(&)[V]>(v[k * V]));
+  }
   __device__ __forceinline__ void get(const float4 *, float (&o)[W]) const {
 #pragma unroll
     for (int j = 0; j < W; ++j) o[j] = v[j];
   }
 };
 template <int W, int TPR> struct ColumnSum<W, TPR, true> {
-  float v[W]; // only between load and save
+  float v[W]; // of vector k only between its load and save
   __device__ __forceinline__ void clear(float4 *lds) {
 #pragma unroll
     for (int j = 0; j < W / 4; ++j) lds[j * TPR + threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  __device__ __forceinline__ void load(float4 *lds) {
+  template <int V> __device__ __forceinline__ void load(float4 *lds, int k) {
 #pragma unroll
-    for (int j = 0; j < W / 4; ++j) {
+    for (int j = k * V / 4; j < (k + 1) * V / 4; ++j) {
       const float4 t = lds[j * TPR + threadIdx.x];
       v[4 * j] = t.x; v[4 * j + 1] = t.y; v[4 * j + 2] = t.z; v[4 * j + 3] = t.w;
     }
   }
   __device__ __forceinline__ void add(float4 *, int j, float a, float b) { v[j] = fmaf(a, b, v[j]); }
-  __device__ __forceinline__ void save(float4 *lds) {
+  template <int V> __device__ __forceinline__ void save(float4 *lds, int k) {
 #pragma unroll
-    for (int j = 0; j < W / 4; ++j)
+    for (int j = k * V / 4; j < (k + 1) * V / 4; ++j)
       lds[j * TPR + threadIdx.x] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
   }
   __device__ __forceinline__ void get(const float4 *lds, float (&o)[W]) const {
@@ -648,33 +678,42 @@ void step_bwd_rows_kernel(const StepArgs a) {
       float t[W];
       if constexpr (PRE) {
         const float rho = in ? inv_std(r.v2, a.eps) : 0.f, mu = r.m2;
-        float s[S], hh[W], d[W];
+        float s[S];
 #pragma unroll
         for (int i = 0; i < S; ++i) s[i] = 0.f;
-        r.h.template unit<LN>(a, mu, rho, hh);
-        P::unpack(r.dy, d);
-        C.load(c_lds);
-        if constexpr (LN) E.load(e_lds);
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-          C.add(c_lds, j, d[j], hh[j]);
-          if constexpr (LN) E.add(e_lds, j, d[j], 1.f);
-          d[j] *= gn[j];
-          if constexpr (LN) s[S - 1] += d[j];
-          s[0] = fmaf(d[j], hh[j], s[0]);
+        for (int k = 0; k < NV; ++k) {
+          float hh[V], d[V];
+          r.h.template unit<LN>(a, mu, rho, k, hh);
+          Tok<T>::unpack(r.dy.p[k], d);
+          C.template load<V>(c_lds, k);
+          if constexpr (LN) E.template load<V>(e_lds, k);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            C.add(c_lds, k * V + j, d[j], hh[j]);
+            if constexpr (LN) E.add(e_lds, k * V + j, d[j], 1.f);
+            d[j] *= gn[k * V + j];
+            if constexpr (LN) s[S - 1] += d[j];
+            s[0] = fmaf(d[j], hh[j], s[0]);
+          }
+          C.template save<V>(c_lds, k);
+          if constexpr (LN) E.template save<V>(e_lds, k);
+          one_vector_at_a_time<NV>();
         }
-        C.save(c_lds);
-        if constexpr (LN) E.save(e_lds);
         r.h.pin();
         r.dy.pin();
         row_total<TPR, S>(s, lds, turn);
         const float s2 = s[0] * inv, s1 = LN ? s[S - 1] * inv : 0.f;
-        r.h.template unit<LN>(a, mu, rho, hh);
-        P::unpack(r.dy, d);
-        P::unpack(r.dh, t);
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-          t[j] = fmaf(rho, fmaf(d[j], gn[j], -(LN ? fmaf(hh[j], s2, s1) : hh[j] * s2)), t[j]);
+        for (int k = 0; k < NV; ++k) {
+          float hh[V], d[V], g[V];
+          r.h.template unit<LN>(a, mu, rho, k, hh);
+          Tok<T>::unpack(r.dy.p[k], d);
+          Tok<T>::unpack(r.dh.p[k], g);
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            t[k * V + j] = fmaf(rho, fmaf(d[j], gn[k * V + j], -(LN ? fmaf(hh[j], s2, s1) : hh[j] * s2)), g[j]);
+          one_vector_at_a_time<NV>();
         }
       } else {
         P::unpack(r.dh, t);
@@ -692,11 +731,16 @@ void step_bwd_rows_kernel(const StepArgs a) {
       float m[S], xh[W];
 #pragma unroll
       for (int i = 0; i < S; ++i) m[i] = 0.f;
-      if constexpr (POST)
-        r.x.template unit<LN>(a, mu, rho, xh);
-      else
-        r.x.get(a, xh);
+      auto get_x = [&](int k) {
+        float(&o)[V] = reinterpret_cast<float(&)[V]>(xh[k * V]);
+        if constexpr (POST)
+          r.x.template unit<LN>(a, mu, rho, k, o);
+        else
+          r.x.get(a, k, o);
+      };
       if constexpr (OPTIONS) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) get_x(k);
         const bool full = a.gate_kind == 2;
         float g[W];
         if constexpr (POST && LN) pl.bias(full ? a.beta_post : nullptr, g);
@@ -710,30 +754,39 @@ void step_bwd_rows_kernel(const StepArgs a) {
         for (int j = 0; j < W; ++j) t[j] *= full ? g[j] : 1.f;
       }
       // branch_scale and a shared gate are multiplied in after the column sums
-      A.load(a_lds);
-      if constexpr (LN && POST) B.load(b_lds);
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        A.add(a_lds, j, t[j], xh[j]);
-        if constexpr (LN && POST) B.add(b_lds, j, t[j], 1.f);
-        t[j] *= kp[j];
-        if constexpr (POST) {
-          if constexpr (LN) m[S - 1] += t[j];
-          m[0] = fmaf(t[j], xh[j], m[0]);
+      for (int k = 0; k < NV; ++k) {
+        if constexpr (!OPTIONS) get_x(k);
+        A.template load<V>(a_lds, k);
+        if constexpr (LN && POST) B.template load<V>(b_lds, k);
+#pragma unroll
+        for (int j = k * V; j < (k + 1) * V; ++j) {
+          A.add(a_lds, j, t[j], xh[j]);
+          if constexpr (LN && POST) B.add(b_lds, j, t[j], 1.f);
+          t[j] *= kp[j];
+          if constexpr (POST) {
+            if constexpr (LN) m[S - 1] += t[j];
+            m[0] = fmaf(t[j], xh[j], m[0]);
+          }
         }
+        A.template save<V>(a_lds, k);
+        if constexpr (LN && POST) B.template save<V>(b_lds, k);
+        one_vector_at_a_time<NV>();
       }
       // (Columns beyond the row's end carry finite leftovers here; their gamma is
       // zero, so no row sum has them, and no sum or element of theirs is stored.)
-      A.save(a_lds);
-      if constexpr (LN && POST) B.save(b_lds);
       if constexpr (POST) {
         if constexpr (PRE) r.x.pin(); // (the first norm alone has registers to keep xh)
         row_total<TPR, S>(m, lds, turn);
         const float s2 = m[0] * inv, s1 = LN ? m[S - 1] * inv : 0.f;
-        if constexpr (PRE) r.x.template unit<LN>(a, mu, rho, xh);
 #pragma unroll
-        for (int j = 0; j < W; ++j)
-          t[j] = rho * (t[j] - (LN ? fmaf(xh[j], s2, s1) : xh[j] * s2));
+        for (int k = 0; k < NV; ++k) {
+          if constexpr (PRE) get_x(k);
+#pragma unroll
+          for (int j = k * V; j < (k + 1) * V; ++j)
+            t[j] = rho * (t[j] - (LN ? fmaf(xh[j], s2, s1) : xh[j] * s2));
+          one_vector_at_a_time<NV>();
+        }
       }
       settle(t);
       ask_post(r, base + D * RPB);

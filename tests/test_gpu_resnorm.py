@@ -101,6 +101,16 @@ def test_two_vectors_per_thread(post, pre, norm, dtype, kept):
         run(Step(10, cols, dtype, norm, post, pre, True, gate, samples=2), kept)
 
 
+@pytest.mark.parametrize("dtype,kept", [("f32", None), ("bf16", None), ("f16", "int8")])
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize("post,pre", [(True, True), (True, False), (False, True)])
+def test_several_wide_rows_per_block(post, pre, norm, dtype, kept):
+    """Rows of two and four vectors per thread, three rows for every CU: a block's
+    rows one after another, their sums carried along."""
+    cols = 4104 if dtype == "f32" else 8200
+    run(Step(600, cols, dtype, norm, post, pre, True, "channel"), kept)
+
+
 @pytest.mark.parametrize("norm", ["rms", "layer"])
 def test_without_parameters(norm):
     run(Step(40, 520, "f16", norm, gate="sample", samples=4, affine=False))
