@@ -14,7 +14,7 @@
 // LayerNormalization 44 + 6 us, 4.6 TB/s; from 8 bits [8192, 4096] bf16 72 + 6 us,
 // 4.7 TB/s.  [2048, 16384] bf16 (four vectors) forward 56, backward 91 + 9 us.
 // Rows that end inside a vector take more instructions and requests: [8191, 4097]
-// bf16 backward 118 us, 3.4 TB/s, where whole rows of that size take 87.
+// bf16 backward 118 us, 3.4 TB/s; whole rows of [16384, 4096] reach 5.0 (160 us).
 // A row's loads are asked for one row ahead and must stay in flight while the
 // row before is worked on and stored.  This GPU counts loads and stores in one
 // in-order counter per wave, and the compiler can wait for "all but the last
