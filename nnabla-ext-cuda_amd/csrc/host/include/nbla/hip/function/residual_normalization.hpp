@@ -33,6 +33,7 @@ protected:
   bool post_, pre_, residual_, gate_;
   float res_scale_, branch_scale_, eps_;
   bool no_scale_, no_bias_;
+  string checkpoint_;
   int format8_;
   Size_t rows_ = 0, cols_ = 0, gate_rows_ = 0;
   int gate_kind_ = NBLAHIP_GATE_NONE;
@@ -53,11 +54,24 @@ public:
       : Function(ctx), device_(std::stoi(ctx.device_id)), batch_axis_(batch_axis), norm_(norm),
         post_(post), pre_(pre), residual_(residual), gate_(gate), res_scale_(res_scale),
         branch_scale_(branch_scale), eps_(eps), no_scale_(no_scale), no_bias_(no_bias),
+        checkpoint_(checkpoint),
         format8_(act8_format(checkpoint)) {}
   virtual ~ResidualNormalizationHip() {}
   virtual string name() { return "ResidualNormalizationHip"; }
   virtual int min_inputs() { return 1; }
   virtual int min_outputs() { return 1; }
+  // What a core asks of a function without a class of its own in it.
+  virtual vector<dtypes> in_types() { return {get_dtype<T>()}; }
+  virtual vector<dtypes> out_types() { return vector<dtypes>(pre_ ? 2 : 1, get_dtype<T>()); }
+  virtual std::shared_ptr<Function> copy() const {
+    return std::make_shared<ResidualNormalizationHip<T>>(
+        this->ctx_, batch_axis_, norm_, post_, pre_, residual_, gate_, res_scale_, branch_scale_, eps_,
+        no_scale_, no_bias_, checkpoint_);
+  }
+  // The backward reads h for the second norm (or its 8-bit copy): it must be kept.
+  virtual bool grad_depends_output_data(int i, int o) const {
+    return pre_ && format8_ == NBLAHIP_ACT8_NONE && o == 0;
+  }
   virtual vector<string> allowed_array_classes() {
     return SingletonManager::get<Hip>()->array_classes();
   }

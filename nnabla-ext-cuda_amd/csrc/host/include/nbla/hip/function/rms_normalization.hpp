@@ -24,6 +24,7 @@ protected:
   vector<int> batch_axis_;
   float eps_;
   bool no_scale_;
+  string checkpoint_;
   int format8_;
   Size_t rows_ = 0, cols_ = 0;
   Variable ms_; // float32 mean squares kept for backward
@@ -36,11 +37,18 @@ public:
   RMSNormalizationHip(const Context &ctx, const vector<int> &batch_axis, float eps, bool no_scale,
                       const string &checkpoint)
       : Function(ctx), device_(std::stoi(ctx.device_id)), batch_axis_(batch_axis), eps_(eps),
-        no_scale_(no_scale), format8_(act8_format(checkpoint)) {}
+        no_scale_(no_scale), checkpoint_(checkpoint),
+        format8_(act8_format(checkpoint)) {}
   virtual ~RMSNormalizationHip() {}
   virtual string name() { return "RMSNormalizationHip"; }
   virtual int min_inputs() { return 1; }
   virtual int min_outputs() { return 1; }
+  // What a core asks of a function without a class of its own in it.
+  virtual vector<dtypes> in_types() { return {get_dtype<T>()}; }
+  virtual vector<dtypes> out_types() { return vector<dtypes>(1, get_dtype<T>()); }
+  virtual std::shared_ptr<Function> copy() const {
+    return std::make_shared<RMSNormalizationHip<T>>(this->ctx_, batch_axis_, eps_, no_scale_, checkpoint_);
+  }
   virtual vector<string> allowed_array_classes() {
     return SingletonManager::get<Hip>()->array_classes();
   }

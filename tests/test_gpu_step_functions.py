@@ -151,6 +151,22 @@ def test_residual_normalization(post, pre, residual, gate, norm, checkpoint, tc)
             assert (np.abs(v.g - twice) <= step * np.abs(twice) * 2 + 2.0 ** -24).all(), names[k]
 
 
+@pytest.mark.parametrize("checkpoint", ["", "int8"])
+def test_no_rows(checkpoint):
+    f = B.RMSNormalization(B.context(), checkpoint=checkpoint)
+    x, g, y = B.Variable((0, 40)), B.Variable((40,)), B.Variable((0, 40))
+    put(g, np.ones(40))
+    f.setup([x, g], [y])
+    f.forward([x, g], [y])
+    f.backward([x, g], [y], [True, True], [False, False])
+    assert (np.asarray(g.g) == 0).all()
+    r = B.ResidualNormalization(B.context(), no_scale=True, checkpoint=checkpoint)
+    res, h, z = B.Variable((0, 40)), B.Variable((0, 40)), B.Variable((0, 40))
+    r.setup([x, res], [h, z])
+    r.forward([x, res], [h, z])
+    r.backward([x, res], [h, z], [True, True], [False, False])
+
+
 def test_the_same_variable_as_block_output_and_residual():
     shape = (9, 64)
     rng = np.random.default_rng(2)
