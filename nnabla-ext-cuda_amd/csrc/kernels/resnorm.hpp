@@ -78,6 +78,7 @@ constexpr int bwd_waves(int vec, bool layer, bool post, bool pre, bool q8, int m
   if (tpr == 1024) return 4;
   if (vec == 4) return mode == kAny && layer && both ? 4 : mode != kWhole || (layer && both) ? 5 : 6;
   if (layer) return (pre ? 4 : 5) - (mode != kWhole ? 1 : 0);
+  if (mode == kRagged && pre && !q8 && (tpr % 192 == 0 || tpr == 640)) return 4; // (bwd_dwords)
   return mode == kWhole ? (pre ? 5 : 6) : mode == kRagged && !(both && q8) ? 5 : 4;
 }
 constexpr int bwd_blocks_per_cu(int vec, bool layer, bool post, bool pre, bool q8, int mode, int tpr, int nv) {

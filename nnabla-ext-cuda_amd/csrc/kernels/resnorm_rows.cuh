@@ -14,7 +14,7 @@
 // LayerNormalization 44 + 6 us, 4.6 TB/s; from 8 bits [8192, 4096] bf16 72 + 6 us,
 // 4.7 TB/s.  [2048, 16384] bf16 (four vectors) forward 56, backward 91 + 9 us.
 // Rows that end inside a vector take more instructions and requests: [8191, 4097]
-// bf16 backward 118 us, 3.4 TB/s; whole rows of [16384, 4096] reach 5.0 (160 us).
+// bf16 backward 103 us, 3.9 TB/s; whole rows of [16384, 4096] reach 5.0 (160 us).
 // A row's loads are asked for one row ahead and must stay in flight while the
 // row before is worked on and stored.  This GPU counts loads and stores in one
 // in-order counter per wave, and the compiler can wait for "all but the last
@@ -31,7 +31,7 @@
 //   kRagged: rows or tensors at any element.  A row that ends inside a vector is
 //            read as the vector that ends where the row ends, shifted down, and
 //            written in pieces of 8, 4 and 2 bytes; nothing outside the row is
-//            touched;
+//            written, and nothing read outside the dwords it lies in;
 //   kAny   : that, a gate per element and accumulation (absent ones cost loads
 //            and stores that the bounds check drops).
 #pragma once
@@ -140,12 +140,17 @@ template <int NV> __device__ __forceinline__ void one_vector_at_a_time() {
 // the first of them: of a tensor of the storage type, of 8-bit codes, of their
 // scales, of a row statistic.  Of ragged rows the thread a row ends in reads the
 // vector `drop` elements further ahead, and writes the first `n` of its own.
-template <typename T, int TPR, int BLOCK, int MODE, int NV> struct Place {
+template <typename T, int TPR, int BLOCK, int MODE, int NV, bool DWORDS = false> struct Place {
   static constexpr int V = Tok<T>::VEC, W = NV * V;
   static constexpr uint32_t SZ = sizeof(T);
   static constexpr bool RAGGED = MODE != kWhole;
+  // DWORDS: 16-bit rows may start in the middle of a dword, where a vector load takes
+  // longer; the dwords that hold the vector are loaded, a fifth one where it straddles
+  // them, and shifted when the vector is used.
+  static constexpr bool HALVES = DWORDS && RAGGED && SZ == 2;
   struct Vec {
     Packed p[NV];
+    uint32_t next[HALVES ? NV : 1], odd; // HALVES: the dword behind; bytes of the row's first dword before it
     // Hides the value from the optimiser, so that its widened form is made anew
     // where it is needed instead of being kept in twice the registers.
     __device__ __forceinline__ void pin() {
@@ -196,14 +201,37 @@ template <typename T, int TPR, int BLOCK, int MODE, int NV> struct Place {
     for (int k = 0; k < NV; ++k) r.p[k] = Tok<T>::pack(reinterpret_cast<const float(&)[V]>(o[k * V]));
     return r;
   }
-  __device__ __forceinline__ Vec load(Buffer b) const {
+  // The thread's vectors of the `bytes` bytes of rows at p + off, to be settled by
+  // fix() when they are used: a load must not be waited for where it is asked for.
+  __device__ __forceinline__ Vec load(const void *p, int64_t off, uint32_t bytes) const {
     Vec r;
+    if constexpr (HALVES) {
+      r.odd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) + off) & 2u;
+      const Buffer b = buffer(p, off - r.odd, bytes ? (bytes + r.odd + 3u) & ~3u : 0u);
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      r.p[k] = buffer_load(b, wide[k]);
-      if constexpr (RAGGED) r.p[k].v = shift_down_bits(r.p[k].v, drop[k] * 8u * SZ);
+      for (int k = 0; k < NV; ++k) {
+        const uint32_t at = wide[k] < bytes ? wide[k] + r.odd : kOutside;
+        r.p[k] = buffer_load(b, at & ~3u);
+        r.next[k] = __builtin_amdgcn_raw_buffer_load_b32(b, at & 2u ? at + 14u : kOutside, 0, 0);
+      }
+    } else {
+      const Buffer b = buffer(p, off, bytes);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) r.p[k] = buffer_load(b, wide[k]);
     }
     return r;
+  }
+  __device__ __forceinline__ void fix(Vec &r) const {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if constexpr (HALVES) {
+        const uint32_t by = ((wide[k] + r.odd) & 2u) * 8u;
+        uint4 &v = r.p[k].v;
+        v = make_uint4(__builtin_amdgcn_alignbit(v.y, v.x, by), __builtin_amdgcn_alignbit(v.z, v.y, by),
+                       __builtin_amdgcn_alignbit(v.w, v.z, by), __builtin_amdgcn_alignbit(r.next[k], v.w, by));
+      }
+      if constexpr (RAGGED) r.p[k].v = shift_down_bits(r.p[k].v, drop[k] * 8u * SZ);
+    }
   }
   // Offset of the first of the thread's own elements, where it starts to write
   // the pieces of a vector that is cut short.
@@ -233,16 +261,18 @@ template <typename T, int TPR, int BLOCK, int MODE, int NV> struct Place {
       }
     }
   }
-  // onto what `old` (a buffer without records: nothing) holds there
-  __device__ __forceinline__ void put(Buffer b, Buffer old, const float (&o)[W]) const {
+  // Rounds o and stores it in the rows at p + off, or adds it to what is there.
+  __device__ __forceinline__ void put(void *p, bool add, int64_t off, uint32_t bytes, const float (&o)[W]) const {
     if constexpr (MODE == kAny) {
       float sum[W];
-      unpack(load(old), sum);
+      Vec old = load(add ? p : nullptr, off, bytes);
+      fix(old);
+      unpack(old, sum);
 #pragma unroll
       for (int j = 0; j < W; ++j) sum[j] += o[j];
-      store(b, pack(sum));
+      store(buffer(p, off, bytes), pack(sum));
     } else {
-      store(b, pack(o));
+      store(buffer(p, off, bytes), pack(o));
     }
   }
   __device__ __forceinline__ uint2 load_codes(Buffer b, int k) const {
@@ -253,11 +283,13 @@ template <typename T, int TPR, int BLOCK, int MODE, int NV> struct Place {
     } else {
       q.x = __builtin_amdgcn_raw_buffer_load_b32(b, codes[k], 0, 0);
     }
+    return q;
+  }
+  __device__ __forceinline__ void fix_codes(uint2 &q, int k) const {
     if constexpr (RAGGED) {
       const uint64_t v = ((static_cast<uint64_t>(q.y) << 32) | q.x) >> (8u * drop[k]);
       q = make_uint2(static_cast<uint32_t>(v), static_cast<uint32_t>(v >> 32));
     }
-    return q;
   }
   __device__ __forceinline__ void store_codes(Buffer b, uint2 q, int k) const {
     const uint32_t all = !RAGGED || n[k] == V ? codes[k] : kOutside;
@@ -348,9 +380,9 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
     auto ask = [&](int u, int64_t base) {
       const int64_t off = base * a.cols * static_cast<int64_t>(sizeof(T));
       const uint32_t bytes = rows_in<RPB>(base, last) * row_bytes;
-      x[u] = pl.load(buffer(a.x, off, bytes));
-      r[u] = pl.load(buffer(a.res, off, bytes));
-      if constexpr (OPTIONS) gf[u] = pl.load(buffer(a.gate_kind == 2 ? a.gate : nullptr, off, bytes));
+      x[u] = pl.load(a.x, off, bytes);
+      r[u] = pl.load(a.res, off, bytes);
+      if constexpr (OPTIONS) gf[u] = pl.load(a.gate_kind == 2 ? a.gate : nullptr, off, bytes);
     };
 #pragma unroll
     for (int u = 0; u < D; ++u) ask(u, first + u * RPB);
@@ -364,6 +396,8 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
       const int64_t off = base * a.cols * static_cast<int64_t>(sizeof(T));
       float h[W], q[W];
       float m1 = 0.f, v1 = 0.f, m2 = 0.f, v2 = 0.f;
+      pl.fix(x[u]);
+      pl.fix(r[u]);
       P::unpack(x[u], h);
       P::unpack(r[u], q);
 #pragma unroll
@@ -382,6 +416,7 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
       if constexpr (COPY) copy(h, a.x8, a.x8_scale);
       float g[W];
       if constexpr (OPTIONS) {
+        pl.fix(gf[u]);
         P::unpack(gf[u], g);
 #pragma unroll
         for (int j = 0; j < W; ++j) g[j] = a.gate_kind == 2 ? g[j] : 1.f;
@@ -469,9 +504,10 @@ template <typename T, bool Q8, typename P> struct Kept {
   typename P::Vec p;
   __device__ __forceinline__ void ask(const StepArgs &a, const void *data, const uint8_t *, int64_t base,
                                       uint32_t rows, const P &pl) {
-    p = pl.load(buffer(data, base * a.cols * static_cast<int64_t>(sizeof(T)),
-                       rows * static_cast<uint32_t>(a.cols) * static_cast<uint32_t>(sizeof(T))));
+    p = pl.load(data, base * a.cols * static_cast<int64_t>(sizeof(T)),
+                rows * static_cast<uint32_t>(a.cols) * static_cast<uint32_t>(sizeof(T)));
   }
+  __device__ __forceinline__ void fix(const P &pl) { pl.fix(p); }
   __device__ __forceinline__ void get(const StepArgs &, int k, float (&o)[V]) const {
     Tok<T>::unpack(p.p[k], o);
   }
@@ -500,6 +536,10 @@ template <typename T, typename P> struct Kept<T, true, P> {
       q[k] = pl.load_codes(codes, k);
       code[k] = __builtin_amdgcn_raw_buffer_load_b8(of, pl.scale[k], 0, 0);
     }
+  }
+  __device__ __forceinline__ void fix(const P &pl) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) pl.fix_codes(q[k], k);
   }
   __device__ __forceinline__ void get(const StepArgs &a, int k, float (&o)[V]) const {
     act8_decode<V>(q[k], code[k], a.format8, o);
@@ -565,12 +605,18 @@ template <int W, int TPR> struct ColumnSum<W, TPR, true> {
   }
 };
 
+// Vector loads in the middle of a dword: worth the dwords and the shifts in the
+// backward of wide rows ([8191, 4097] bf16 RMS step 128 -> 109 us, [8191, 2049] 81 ->
+// 67), not for two sums per norm (no gain), short rows ([8191, 1023] half 27.7 ->
+// 29.5) and in the forward (68 -> 80), whose time the extra instructions are.
+constexpr bool bwd_dwords(bool layer, int mode, int tpr) { return !layer && mode == kRagged && tpr >= 192; }
+
 // Backward.  Each input vector is asked for again, for the next row, right
 // after its last use.
 template <typename T, bool LN, bool POST, bool PRE, bool Q8, int MODE, int TPR, int NV>
 __global__ __launch_bounds__(bwd_block(TPR), bwd_bound(Tok<T>::VEC, LN, POST, PRE, Q8, MODE, TPR, NV))
 void step_bwd_rows_kernel(const StepArgs a) {
-  using P = Place<T, TPR, bwd_block(TPR), MODE, NV>;
+  using P = Place<T, TPR, bwd_block(TPR), MODE, NV, bwd_dwords(LN, MODE, TPR)>;
   using Vec = typename P::Vec;
   constexpr int V = P::V, W = P::W;
   constexpr bool OPTIONS = MODE == kAny;
@@ -643,18 +689,18 @@ void step_bwd_rows_kernel(const StepArgs a) {
       const int64_t off = base * a.cols * static_cast<int64_t>(sizeof(T));
       if constexpr (PRE) {
         r.h.ask(a, a.kept_h, a.kept_h_scale, base, rows, pl);
-        r.dy = pl.load(buffer(a.dy, off, rows * row_bytes));
+        r.dy = pl.load(a.dy, off, rows * row_bytes);
         if constexpr (LN) r.m2 = buffer_load_float(buffer(a.mean_pre, 4 * base, 4 * rows), pl.stat);
         r.v2 = buffer_load_float(buffer(a.var_pre, 4 * base, 4 * rows), pl.stat);
       }
-      r.dh = pl.load(buffer(a.dh, off, rows * row_bytes));
+      r.dh = pl.load(a.dh, off, rows * row_bytes);
     };
     auto ask_post = [&](Row &r, int64_t base) {
       const uint32_t rows = rows_in<RPB>(base, last);
       r.x.ask(a, a.x, a.kept_x_scale, base, rows, pl);
       if constexpr (OPTIONS)
-        r.gf = pl.load(buffer(a.gate_kind == 2 ? a.gate : nullptr,
-                            base * a.cols * static_cast<int64_t>(sizeof(T)), rows * row_bytes));
+        r.gf = pl.load(a.gate_kind == 2 ? a.gate : nullptr, base * a.cols * static_cast<int64_t>(sizeof(T)),
+                       rows * row_bytes);
       if constexpr (POST) {
         if constexpr (LN) r.m1 = buffer_load_float(buffer(a.mean_post, 4 * base, 4 * rows), pl.stat);
         r.v1 = buffer_load_float(buffer(a.var_post, 4 * base, 4 * rows), pl.stat);
@@ -679,6 +725,8 @@ void step_bwd_rows_kernel(const StepArgs a) {
       if constexpr (PRE) {
         const float rho = in ? inv_std(r.v2, a.eps) : 0.f, mu = r.m2;
         float s[S];
+        r.h.fix(pl);
+        pl.fix(r.dy);
 #pragma unroll
         for (int i = 0; i < S; ++i) s[i] = 0.f;
 #pragma unroll
@@ -704,6 +752,7 @@ void step_bwd_rows_kernel(const StepArgs a) {
         r.dy.pin();
         row_total<TPR, S>(s, lds, turn);
         const float s2 = s[0] * inv, s1 = LN ? s[S - 1] * inv : 0.f;
+        pl.fix(r.dh);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
           float hh[V], d[V], g[V];
@@ -716,6 +765,7 @@ void step_bwd_rows_kernel(const StepArgs a) {
           one_vector_at_a_time<NV>();
         }
       } else {
+        pl.fix(r.dh);
         P::unpack(r.dh, t);
       }
       settle(t);
@@ -724,11 +774,11 @@ void step_bwd_rows_kernel(const StepArgs a) {
         float o[W];
 #pragma unroll
         for (int j = 0; j < W; ++j) o[j] = a.res_scale * t[j];
-        pl.put(buffer(a.dres, off, rows * row_bytes),
-               buffer(a.accum & NBLAHIP_ACCUM_DRES ? a.dres : nullptr, off, rows * row_bytes), o);
+        pl.put(a.dres, a.accum & NBLAHIP_ACCUM_DRES, off, rows * row_bytes, o);
       }
       const float rho = POST ? in ? inv_std(r.v1, a.eps) : 0.f : 1.f, mu = POST ? r.m1 : 0.f;
       float m[S], xh[W];
+      r.x.fix(pl);
 #pragma unroll
       for (int i = 0; i < S; ++i) m[i] = 0.f;
       auto get_x = [&](int k) {
@@ -747,8 +797,8 @@ void step_bwd_rows_kernel(const StepArgs a) {
 #pragma unroll
         for (int j = 0; j < W; ++j)
           g[j] = t[j] * (POST && LN ? fmaf(xh[j], kp[j], a.branch_scale * g[j]) : xh[j] * kp[j]);
-        pl.put(buffer(full ? a.dgate : nullptr, off, rows * row_bytes),
-               buffer(full && (a.accum & NBLAHIP_ACCUM_DGATE) ? a.dgate : nullptr, off, rows * row_bytes), g);
+        pl.put(full ? a.dgate : nullptr, a.accum & NBLAHIP_ACCUM_DGATE, off, rows * row_bytes, g);
+        pl.fix(r.gf);
         P::unpack(r.gf, g);
 #pragma unroll
         for (int j = 0; j < W; ++j) t[j] *= full ? g[j] : 1.f;
@@ -790,8 +840,7 @@ void step_bwd_rows_kernel(const StepArgs a) {
       }
       settle(t);
       ask_post(r, base + D * RPB);
-      pl.put(buffer(a.dx, off, rows * row_bytes),
-             buffer(a.accum & NBLAHIP_ACCUM_DX ? a.dx : nullptr, off, rows * row_bytes), t);
+      pl.put(a.dx, a.accum & NBLAHIP_ACCUM_DX, off, rows * row_bytes, t);
      }
     }
     if (a.part_post) {
