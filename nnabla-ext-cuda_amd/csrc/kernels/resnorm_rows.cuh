@@ -449,10 +449,9 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
         moments(m1, v1);
         rho = inv_std(v1, a.eps);
       }
-      const float shift1 = -m1 * rho; // 16-bit data: see Kept::unit
 #pragma unroll
       for (int j = 0; j < W; ++j) {
-        const float xh = !(POST && LN) ? h[j] * rho : V == 8 ? fmaf(h[j], rho, shift1) : (h[j] - m1) * rho;
+        const float xh = (POST && LN ? h[j] - m1 : h[j]) * rho;
         if constexpr (OPTIONS) {
           h[j] = fmaf(POST && LN ? fmaf(xh, kp[j], kb[j]) : xh * kp[j], g[j], q[j]);
         } else {
@@ -469,7 +468,7 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
       }
       if constexpr (PRE) {
         moments(m2, v2);
-        const float rho2 = inv_std(v2, a.eps), shift2 = -m2 * rho2;
+        const float rho2 = inv_std(v2, a.eps);
         float y[W];
 #pragma unroll
         for (int j = 0; j < W; ++j) {
@@ -480,8 +479,7 @@ __global__ __launch_bounds__(fwd_block(TPR)) void step_fwd_rows_kernel(const Ste
               bn[j] = b.x; bn[j + 1] = b.y; bn[j + 2] = b.z; bn[j + 3] = b.w;
             }
           }
-          y[j] = !LN ? h[j] * rho2 * gn[j]
-                     : fmaf(V == 8 ? fmaf(h[j], rho2, shift2) : (h[j] - m2) * rho2, gn[j], bn[j]);
+          y[j] = LN ? fmaf((h[j] - m2) * rho2, gn[j], bn[j]) : h[j] * rho2 * gn[j];
         }
         pl.store(buffer(a.y, off, bytes), P::pack(y));
       }
@@ -511,15 +509,13 @@ template <typename T, bool Q8, typename P> struct Kept {
   __device__ __forceinline__ void get(const StepArgs &, int k, float (&o)[V]) const {
     Tok<T>::unpack(p.p[k], o);
   }
-  // (value - mu) * rho.  16-bit data takes one fma, value * rho - mu * rho: off by
-  // 2^-24 |mu| rho, far below what the data resolves; float data is centred first.
+  // (value - mu) * rho, centred first: value * rho - mu * rho would carry the rounding
+  // of mu * rho, 2^-24 of a value far from zero, into the float column sums.
   template <bool CENTRED>
   __device__ __forceinline__ void unit(const StepArgs &a, float mu, float rho, int k, float (&o)[V]) const {
     get(a, k, o);
-    const float shift = -mu * rho;
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      o[j] = !CENTRED ? o[j] * rho : sizeof(T) == 2 ? fmaf(o[j], rho, shift) : (o[j] - mu) * rho;
+    for (int j = 0; j < V; ++j) o[j] = (CENTRED ? o[j] - mu : o[j]) * rho;
   }
   __device__ __forceinline__ void pin() { p.pin(); }
 };
@@ -544,13 +540,14 @@ template <typename T, typename P> struct Kept<T, true, P> {
   __device__ __forceinline__ void get(const StepArgs &a, int k, float (&o)[V]) const {
     act8_decode<V>(q[k], code[k], a.format8, o);
   }
-  // One multiplication takes the scale (a power of two: exact) and rho.
+  // Centred by one fma with the scale (a power of two: the product is exact); without
+  // a mean one multiplication takes scale and rho.
   template <bool CENTRED>
   __device__ __forceinline__ void unit(const StepArgs &a, float mu, float rho, int k, float (&o)[V]) const {
-    const float shift = -mu * rho, scale = act8_scale(code[k]) * rho;
+    const float scale = CENTRED ? act8_scale(code[k]) : act8_scale(code[k]) * rho;
     act8_numbers<V>(q[k], a.format8, o);
 #pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = CENTRED ? fmaf(o[j], scale, shift) : o[j] * scale;
+    for (int j = 0; j < V; ++j) o[j] = CENTRED ? fmaf(o[j], scale, -mu) * rho : o[j] * scale;
   }
   __device__ __forceinline__ void pin() {
 #pragma unroll
