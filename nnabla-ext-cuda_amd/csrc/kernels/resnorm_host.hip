@@ -119,7 +119,7 @@ size_t plan_bwd(StepArgs &a, StepPlan &pl, int64_t gate_rows, char *ws) {
   });
   a.pitch = (a.cols + 7) / 8 * 8;
   if (pl.tpr == 0) {
-    plan_chunks(a, gate_rows, kCus, 16);
+    plan_chunks(a, gate_rows, std::max<int64_t>(kCus, (a.rows + kLongRun - 1) / kLongRun), 16);
     a.grid = a.chunks;
   } else {
     const int block = bwd_block(pl.tpr);
@@ -170,17 +170,34 @@ __device__ __forceinline__ float4 fold_rows(const float *p, int64_t n, int64_t s
                                             const float *weight, int64_t per, int64_t cols, int64_t c,
                                             int nc, float4 *lds) {
   const int row = threadIdx.x / kFoldLanes, lane = threadIdx.x % kFoldLanes;
-  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int64_t r = row; r < n; r += kFoldRows) {
-    float4 v = *reinterpret_cast<const float4 *>(p + r * stride + c);
+  // Four rows in float, those in double: a gate row per token leaves a row per token,
+  // and equal values added up one by one are rounded the same way each time.
+  double sum[4] = {0., 0., 0., 0.};
+  const int64_t step = kFoldRows * stride;
+  const float *at = p + row * stride + c;
+  auto load = [&](int64_t r, const float *from) {
+    float4 v = *reinterpret_cast<const float4 *>(from);
     if (weight) {
       float w[4];
       load_param<4>(weight, r / per * cols + c, nc, w);
       v.x *= w[0]; v.y *= w[1]; v.z *= w[2]; v.w *= w[3];
     }
-    s = add4(s, v);
+    return v;
+  };
+  int64_t r = row;
+  for (; r + 3 * kFoldRows < n; r += 4 * kFoldRows, at += 4 * step) {
+    float4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = load(r + i * kFoldRows, at + i * step);
+    const float4 t = add4(add4(v[0], v[1]), add4(v[2], v[3]));
+    sum[0] += t.x; sum[1] += t.y; sum[2] += t.z; sum[3] += t.w;
   }
+  for (; r < n; r += kFoldRows, at += step) {
+    const float4 t = load(r, at);
+    sum[0] += t.x; sum[1] += t.y; sum[2] += t.z; sum[3] += t.w;
+  }
+  float4 s = make_float4(static_cast<float>(sum[0]), static_cast<float>(sum[1]),
+                         static_cast<float>(sum[2]), static_cast<float>(sum[3]));
   __syncthreads();
   lds[threadIdx.x] = s;
   __syncthreads();

@@ -11,12 +11,27 @@
 // sums, 109 for the rest, 11 for the fold).
 #pragma once
 
+#include <type_traits>
+
 #include "resnorm.hpp"
 #include "tokens.cuh"
 
 namespace nblahip {
 
 constexpr int kLongThreads = 512;
+
+// A thread's share of a row sum: a vector's part in float, the vectors' in double.
+// In float the share would be one chain of additions, each of equal values rounded the
+// same way: off by 6e-5 for 8192 times 0.1 (a row of 2^22 columns), 2.5e-3 for 2^18.
+// One conversion and one addition per vector do not show beside its memory accesses.
+template <int N> struct RowShare {
+  double s[N] = {};
+  __device__ __forceinline__ void add(int i, float v) { s[i] += static_cast<double>(v); }
+  __device__ __forceinline__ void get(float (&o)[N]) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = static_cast<float>(s[i]);
+  }
+};
 
 // Sum of N values over the block; every thread returns the same sums.
 template <int N> __device__ __forceinline__ void long_sum(float (&v)[N]) {
@@ -77,27 +92,33 @@ __device__ __forceinline__ void long_moments(int64_t cols, F f, float &mean, flo
   const float inv = 1.f / static_cast<float>(cols);
   mean = 0.f;
   if constexpr (LN) {
-    float s[1] = {0.f};
+    RowShare<1> share;
     for (int64_t c = threadIdx.x * V; c < cols; c += kLongThreads * V) {
-      float v[V];
+      float v[V], t = 0.f;
       f(c, columns_left(cols - c, V), v);
 #pragma unroll
-      for (int j = 0; j < V; ++j) s[0] += v[j];
+      for (int j = 0; j < V; ++j) t += v[j];
+      share.add(0, t);
     }
+    float s[1];
+    share.get(s);
     long_sum<1>(s);
     mean = s[0] * inv;
   }
-  float s[1] = {0.f};
+  RowShare<1> share;
   for (int64_t c = threadIdx.x * V; c < cols; c += kLongThreads * V) {
-    float v[V];
+    float v[V], t = 0.f;
     const int n = columns_left(cols - c, V);
     f(c, n, v);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const float d = j < n ? v[j] - mean : 0.f;
-      s[0] = fmaf(d, d, s[0]);
+      t = fmaf(d, d, t);
     }
+    share.add(0, t);
   }
+  float s[1];
+  share.get(s);
   long_sum<1>(s);
   var = s[0] * inv;
 }
@@ -221,36 +242,46 @@ __device__ __forceinline__ void long_dh(const StepArgs &a, int64_t row, int64_t 
 }
 
 // Row sums of the backward: row_sums[row] = {s1, s2, m1, m2}, the two means of
-// each norm's backward.
+// each norm's backward.  The half RMS step from its tensors is held to the 80
+// registers of six waves per SIMD, which it fits; left alone it takes 81 and runs
+// five ([700, 40001] 86 -> 90 us).  The other forms of 80 and more would spill.
+template <typename T, bool LN, bool Q8>
+constexpr int kLongSumsWaves = std::is_same<T, __half>::value && !LN && !Q8 ? 6 : 1;
 template <typename T, bool LN, bool POST, bool PRE, bool Q8>
-__global__ __launch_bounds__(kLongThreads) void step_bwd_long_sums_kernel(const StepArgs a) {
+__global__ __launch_bounds__(kLongThreads, (kLongSumsWaves<T, LN, Q8>))
+void step_bwd_long_sums_kernel(const StepArgs a) {
   constexpr int V = Tok<T>::VEC;
   const float inv = 1.f / static_cast<float>(a.cols);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const RowMoments q = load_moments<LN, POST, PRE>(a, row);
     float s[2] = {0.f, 0.f}, m[2] = {0.f, 0.f};
     if constexpr (PRE) {
+      RowShare<2> share;
       for (int64_t c = threadIdx.x * V; c < a.cols; c += kLongThreads * V) {
         const int n = columns_left(a.cols - c, V);
-        float hh[V], dy[V], ga[V];
+        float hh[V], dy[V], ga[V], g0 = 0.f, g1 = 0.f;
         load_kept<T, Q8>(a.kept_h, a.kept_h_scale, a, row, c, n, hh);
         Tok<T>::unpack(Tok<T>::load(static_cast<const T *>(a.dy) + row * a.cols + c, n), dy);
         load_param<V>(a.gamma_pre, c, n, ga);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const float g = dy[j] * ga[j];
-          if constexpr (LN) s[0] += g;
-          s[1] = fmaf(g, j < n ? (hh[j] - q.m2) * q.r2 : 0.f, s[1]);
+          if constexpr (LN) g0 += g;
+          g1 = fmaf(g, j < n ? (hh[j] - q.m2) * q.r2 : 0.f, g1);
         }
+        if constexpr (LN) share.add(0, g0);
+        share.add(1, g1);
       }
+      share.get(s);
       long_sum<2>(s);
       s[0] *= inv;
       s[1] *= inv;
     }
     if constexpr (POST) {
+      RowShare<2> share;
       for (int64_t c = threadIdx.x * V; c < a.cols; c += kLongThreads * V) {
         const int n = columns_left(a.cols - c, V);
-        float t[V], hh[V], dy[V], xh[V], g[V], ga[V];
+        float t[V], hh[V], dy[V], xh[V], g[V], ga[V], w0 = 0.f, w1 = 0.f;
         long_dh<T, LN, PRE, Q8>(a, row, c, n, q, s[0], s[1], t, hh, dy);
         load_kept<T, Q8>(a.x, a.kept_x_scale, a, row, c, n, xh);
         load_gate<T>(a, row, c, n, g);
@@ -258,10 +289,13 @@ __global__ __launch_bounds__(kLongThreads) void step_bwd_long_sums_kernel(const 
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const float w = a.branch_scale * t[j] * g[j] * ga[j];
-          if constexpr (LN) m[0] += w;
-          m[1] = fmaf(w, j < n ? (xh[j] - q.m1) * q.r1 : 0.f, m[1]);
+          if constexpr (LN) w0 += w;
+          w1 = fmaf(w, j < n ? (xh[j] - q.m1) * q.r1 : 0.f, w1);
         }
+        if constexpr (LN) share.add(0, w0);
+        share.add(1, w1);
       }
+      share.get(m);
       long_sum<2>(m);
       m[0] *= inv;
       m[1] *= inv;
@@ -273,7 +307,8 @@ __global__ __launch_bounds__(kLongThreads) void step_bwd_long_sums_kernel(const 
 
 // Everything else: a block takes one run of rows with one gate row at
 // kLongThreads vectors' worth of columns, writes dx, dres and a full gate's
-// gradient, and leaves the run's column sums.
+// gradient, and leaves the run's column sums (of at most kLongRun rows, one after
+// another).
 template <typename T, bool LN, bool POST, bool PRE, bool Q8>
 __global__ __launch_bounds__(kLongThreads) void step_bwd_long_cols_kernel(const StepArgs a) {
   constexpr int V = Tok<T>::VEC;
