@@ -123,6 +123,13 @@ NNABLA_HIP_EXPORT nnabla_hip_function *nnabla_hip_create_residual_normalization(
 NNABLA_HIP_EXPORT void nnabla_hip_function_delete(nnabla_hip_function *f);
 NNABLA_HIP_EXPORT const char *nnabla_hip_function_name(nnabla_hip_function *f);
 
+/* Whether the gradient of input i reads the data of input j / of output o, which
+ * must then be kept from the forward to the backward. */
+NNABLA_HIP_EXPORT int nnabla_hip_function_grad_depends_input_data(nnabla_hip_function *f, int i,
+                                                                  int j, int *depends);
+NNABLA_HIP_EXPORT int nnabla_hip_function_grad_depends_output_data(nnabla_hip_function *f, int i,
+                                                                   int o, int *depends);
+
 /* Function::setup / forward / backward / recompute. */
 NNABLA_HIP_EXPORT int nnabla_hip_function_setup(nnabla_hip_function *f,
                                                 nnabla_hip_variable **inputs, int n_inputs,

@@ -54,6 +54,8 @@ SIGNATURES = {
                                                  [_I, _I, _S]),
     "nnabla_hip_function_delete": (None, [_P]),
     "nnabla_hip_function_name": (_S, [_P]),
+    "nnabla_hip_function_grad_depends_input_data": (_I, [_P, _I, _I, _IP]),
+    "nnabla_hip_function_grad_depends_output_data": (_I, [_P, _I, _I, _IP]),
     "nnabla_hip_function_setup": (_I, [_P, _PP, _I, _PP, _I]),
     "nnabla_hip_function_forward": (_I, [_P, _PP, _I, _PP, _I]),
     "nnabla_hip_function_recompute": (_I, [_P, _PP, _I, _PP, _I]),
@@ -281,6 +283,18 @@ class Function:
     @property
     def name(self):
         return lib().nnabla_hip_function_name(self._h).decode()
+
+    def grad_depends_input_data(self, i, j):
+        """Whether the gradient of input i reads the data of input j."""
+        d = ctypes.c_int()
+        _check(lib().nnabla_hip_function_grad_depends_input_data(self._h, i, j, ctypes.byref(d)))
+        return bool(d.value)
+
+    def grad_depends_output_data(self, i, o):
+        """Whether the gradient of input i reads the data of output o."""
+        d = ctypes.c_int()
+        _check(lib().nnabla_hip_function_grad_depends_output_data(self._h, i, o, ctypes.byref(d)))
+        return bool(d.value)
 
     def setup(self, inputs, outputs):
         i, ni = _handles(inputs)

@@ -582,6 +582,10 @@ public:
   virtual int min_inputs() { return 1; }
   virtual int min_outputs() { return 1; }
   Context context() const { return ctx_; }
+  // Whether the gradient of input i reads the data of output o / of input j: what
+  // a graph asks before it frees data between forward and backward.
+  virtual bool grad_depends_output_data(int i, int o) const { return false; }
+  bool grad_depends_input_data(int i, int j) const { return grad_depends_input_data_impl(i, j); }
 
   void setup(const Variables &inputs, const Variables &outputs) {
     if (fall_back_func_) fall_back_func_.reset();
@@ -625,6 +629,7 @@ protected:
   virtual void recompute_impl(const Variables &inputs, const Variables &outputs) {
     forward_impl(inputs, outputs);
   }
+  virtual bool grad_depends_input_data_impl(int i, int j) const { return true; }
 };
 typedef shared_ptr<Function> FunctionPtr;
 

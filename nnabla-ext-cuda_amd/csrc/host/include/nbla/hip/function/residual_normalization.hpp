@@ -37,7 +37,8 @@ protected:
   int format8_;
   Size_t rows_ = 0, cols_ = 0, gate_rows_ = 0;
   int gate_kind_ = NBLAHIP_GATE_NONE;
-  // positions in the inputs, -1: not there
+  // number of inputs, and positions in them, -1: not there
+  int n_inputs_ = 1;
   int i_res_ = -1, i_gate_ = -1, i_beta_post_ = -1, i_gamma_post_ = -1, i_beta_pre_ = -1,
       i_gamma_pre_ = -1;
   Variable mean_post_, var_post_, mean_pre_, var_pre_; // float32, kept for backward
@@ -54,8 +55,9 @@ public:
       : Function(ctx), device_(std::stoi(ctx.device_id)), batch_axis_(batch_axis), norm_(norm),
         post_(post), pre_(pre), residual_(residual), gate_(gate), res_scale_(res_scale),
         branch_scale_(branch_scale), eps_(eps), no_scale_(no_scale), no_bias_(no_bias),
-        checkpoint_(checkpoint),
-        format8_(act8_format(checkpoint)) {}
+        checkpoint_(checkpoint), format8_(act8_format(checkpoint)) {
+    place_inputs();
+  }
   virtual ~ResidualNormalizationHip() {}
   virtual string name() { return "ResidualNormalizationHip"; }
   virtual int min_inputs() { return 1; }
@@ -83,6 +85,14 @@ protected:
                              const vector<bool> &propagate_down, const vector<bool> &accum);
   void backward_pass(const Variables &inputs, const Variables &outputs,
                      const vector<bool> &propagate_down, const vector<bool> &accum);
+  void place_inputs();
+  // The backward reads the gate, the gammas, a gated step's first beta and, without a
+  // checkpoint, x for the first norm or the gate; everything else may be freed.
+  virtual bool grad_depends_input_data_impl(int i, int j) const {
+    if (j == 0) return reads_x() && format8_ == NBLAHIP_ACT8_NONE;
+    if (j == i_res_ || j == i_beta_pre_) return false;
+    return j == i_beta_post_ ? gate_ : true;
+  }
   bool reads_x() const { return post_ || gate_; }
 };
 } // namespace nbla

@@ -58,5 +58,9 @@ protected:
   virtual void forward_impl(const Variables &inputs, const Variables &outputs);
   virtual void backward_impl(const Variables &inputs, const Variables &outputs,
                              const vector<bool> &propagate_down, const vector<bool> &accum);
+  // With a checkpoint the backward reads the copy: x may be freed after the forward.
+  virtual bool grad_depends_input_data_impl(int i, int j) const {
+    return j == 0 ? format8_ == NBLAHIP_ACT8_NONE : true;
+  }
 };
 } // namespace nbla

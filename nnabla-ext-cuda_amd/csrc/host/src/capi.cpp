@@ -408,6 +408,22 @@ void nnabla_hip_function_delete(nnabla_hip_function *f) { delete f; }
 
 const char *nnabla_hip_function_name(nnabla_hip_function *f) { return f ? f->name.c_str() : ""; }
 
+int nnabla_hip_function_grad_depends_input_data(nnabla_hip_function *f, int i, int j, int *depends) {
+  return guarded([&] {
+    NBLA_CHECK(f, error_code::value, "null function handle");
+    NBLA_CHECK(depends, error_code::value, "depends is null");
+    *depends = f->fn->grad_depends_input_data(i, j);
+  });
+}
+
+int nnabla_hip_function_grad_depends_output_data(nnabla_hip_function *f, int i, int o, int *depends) {
+  return guarded([&] {
+    NBLA_CHECK(f, error_code::value, "null function handle");
+    NBLA_CHECK(depends, error_code::value, "depends is null");
+    *depends = f->fn->grad_depends_output_data(i, o);
+  });
+}
+
 int nnabla_hip_function_setup(nnabla_hip_function *f, nnabla_hip_variable **inputs, int n_inputs,
                               nnabla_hip_variable **outputs, int n_outputs) {
   return guarded([&] {

@@ -6,11 +6,7 @@
 
 namespace nbla {
 
-template <typename T>
-void ResidualNormalizationHip<T>::setup_impl(const Variables &inputs, const Variables &outputs) {
-  NBLA_CHECK(norm_ == "rms" || norm_ == "layer", error_code::value,
-             "norm must be \"rms\" or \"layer\" (given \"%s\").", norm_.c_str());
-  NBLA_CHECK(post_ || pre_, error_code::value, "ResidualNormalization needs post, pre or both.");
+template <typename T> void ResidualNormalizationHip<T>::place_inputs() {
   const bool layer = norm_ == "layer";
   int n = 1;
   auto take = [&](bool there) { return there ? n++ : -1; };
@@ -20,8 +16,17 @@ void ResidualNormalizationHip<T>::setup_impl(const Variables &inputs, const Vari
   i_gamma_post_ = take(post_ && !no_scale_);
   i_beta_pre_ = take(pre_ && layer && !no_bias_);
   i_gamma_pre_ = take(pre_ && !no_scale_);
-  NBLA_CHECK(static_cast<int>(inputs.size()) == n, error_code::value,
-             "ResidualNormalization expects %d inputs, given %zu.", n, inputs.size());
+  n_inputs_ = n;
+}
+
+template <typename T>
+void ResidualNormalizationHip<T>::setup_impl(const Variables &inputs, const Variables &outputs) {
+  NBLA_CHECK(norm_ == "rms" || norm_ == "layer", error_code::value,
+             "norm must be \"rms\" or \"layer\" (given \"%s\").", norm_.c_str());
+  NBLA_CHECK(post_ || pre_, error_code::value, "ResidualNormalization needs post, pre or both.");
+  const bool layer = norm_ == "layer";
+  NBLA_CHECK(static_cast<int>(inputs.size()) == n_inputs_, error_code::value,
+             "ResidualNormalization expects %d inputs, given %zu.", n_inputs_, inputs.size());
   NBLA_CHECK(outputs.size() == (pre_ ? 2u : 1u), error_code::value,
              "ResidualNormalization has %d output(s).", pre_ ? 2 : 1);
   const Shape_t shape = inputs[0]->shape();
@@ -136,7 +141,8 @@ void ResidualNormalizationHip<T>::backward_pass(const Variables &inputs, const V
   const void *gate = nullptr;
   if (gate_kind_ == NBLAHIP_GATE_FULL) gate = inputs[i_gate_]->get_data_pointer<T>(ctx);
   if (gate_kind_ == NBLAHIP_GATE_ROWS) gate = param(i_gate_);
-  const float *bp = param(i_beta_post_), *gp = param(i_gamma_post_), *gn = param(i_gamma_pre_);
+  const float *bp = gate_ ? param(i_beta_post_) : nullptr; // (for the gate's gradient alone)
+  const float *gp = param(i_gamma_post_), *gn = param(i_gamma_pre_);
   const void *x = nullptr, *h = nullptr;
   const uint8_t *xs = nullptr, *hs = nullptr;
   if (format8_) {
