@@ -424,7 +424,7 @@ NBLAHIP_EXPORT int nblahip_in_cl_bwd(const void *x, const void *dy,
  *
  * Tensors are [rows, cols], contiguous, a row per token; dtype is NBLAHIP_F32,
  * NBLAHIP_F16 or NBLAHIP_BF16.  Any number of rows and columns (cols below
- * 2^27, fewer than 2^46 elements; more: NBLAHIP_ERANGE) at element alignment.  Parameters, shared
+ * 2^27, up to 2^46 elements; more: NBLAHIP_ERANGE) at element alignment.  Parameters, shared
  * gates, statistics and their gradients are float32, all arithmetic too; each
  * output is rounded once.  The norms are over the columns:
  *   RMS   : v / sqrt(mean(v^2) + eps) * gamma               (saved: mean square)

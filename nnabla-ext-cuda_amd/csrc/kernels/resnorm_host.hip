@@ -98,7 +98,8 @@ bool whole_vectors(int dtype, int64_t cols, std::initializer_list<const void *> 
 
 // Runs of rows for the backward: rows that share a gate row are cut into
 // chunks_per_gate runs of chunk_rows, so that a run has one gate row and its
-// column sums are one partial sum.
+// column sums are one partial sum.  (Rounded up: with several gate rows the runs may
+// pass the blocks, and some blocks walk two.)
 void plan_chunks(StepArgs &a, int64_t gate_rows, int64_t want_chunks, int64_t min_rows) {
   a.rows_per_gate = std::max<int64_t>(1, a.rows / gate_rows);
   int64_t per = std::max<int64_t>(1, (want_chunks + gate_rows - 1) / gate_rows);
@@ -145,9 +146,9 @@ size_t plan_bwd(StepArgs &a, StepPlan &pl, int64_t gate_rows, char *ws) {
 // partial row): 8 threads of 4 columns by 64 rows.  blockIdx.y: 0 / 1 the second
 // norm's gamma / beta, 2 / 3 the first norm's (a shared gate's rows multiplied
 // in), 4 + g gate row g.  The order of the additions is fixed by the sizes.
-// Bound by its launch and the latency of a thread's reads one after another: 4 - 6
+// Bound by its launch and the latency of a thread's reads, four at a time: 4 - 6.5
 // us for the 2 - 8 MB that most calls leave ([16384, 1024] half with 32 gate rows:
-// 6.1), 11 us for two LayerNormalizations of 16384 columns.
+// 6.2), 11 us for two LayerNormalizations of 16384 columns.
 // ---------------------------------------------------------------------------
 constexpr int kFoldLanes = 8, kFoldRows = 64;
 

@@ -5,10 +5,12 @@
 // bwd_row_fits and fwd_row_fits name.
 //
 // Bound by HBM and, on the way there, by reading twice: the forward's later
-// passes find the row in the caches ([2048, 16384] bf16 step of two
-// LayerNormalizations 119 us, 2.4 times its bytes' time), the backward's two
-// kernels each read every tensor (the same step 196 us, 2.6 times: 74 for the row
-// sums, 109 for the rest, 11 for the fold).
+// passes find the row in the caches ([512, 50000] float step of two
+// LayerNormalizations 162 us, 2.1 times its bytes' time), the backward's two
+// kernels each read every tensor ([2048, 16384] bf16, the same step, 196 - 204 us, 2.6
+// times: 74 for the row sums, 109 - 114 for the rest, 11 for the fold).  Rows of less
+// than a vector keep one thread of a block busy: [200000, 7] half RMS 980 us forward,
+// 1460 backward, where rows of 8 take 13 and 20 (resnorm_rows.cuh).
 #pragma once
 
 #include <type_traits>

@@ -32,8 +32,8 @@
 //            read as the vector that ends where the row ends, shifted down, and
 //            written in pieces of 8, 4 and 2 bytes; nothing outside the row is
 //            written, and nothing read outside the dwords it lies in;
-//   kAny   : that, a gate per element and accumulation (absent ones cost loads
-//            and stores that the bounds check drops).
+//   kAny   : that, a gate per element and accumulation, whole rows too (absent ones
+//            cost loads and stores that the bounds check drops).
 #pragma once
 
 #include "resnorm_long.cuh"
