@@ -128,3 +128,24 @@ def test_a_gate_row_per_token(spread, cols):
     check(g.dgamma_post, terms.sum(0), 24 * U * np.abs(terms).sum(0), "dgamma")
     want = each * f64(gamma)
     check(g.dgate, want, 24 * U * np.abs(want), "dgate")
+
+
+def test_more_runs_of_rows_than_a_grid_has_blocks():
+    rows = 65536 * 256 + 3
+    dy = torch.full((rows, 1), 0.1, dtype=torch.bfloat16, device="cuda")
+    x = torch.full((rows, 1), 2.0, dtype=torch.bfloat16, device="cuda")
+    dy[-3:] = 64.0
+    mean, var = torch.zeros(rows, device="cuda"), torch.ones(rows, device="cuda")
+    g = K.resnorm_backward(x, x, None, dy, (mean, var, mean, var), rows, norm="layer", post=False)
+    rho = 1 / np.sqrt(1 + float(np.float32(1e-5)))
+    want = dy.double().sum().item()
+    check(g.dbeta_pre, [want], COLUMN * want, "dbeta")
+    check(g.dgamma_pre, [want * 2 * rho], COLUMN * want * 2 * rho, "dgamma")
+    # one column: G - mean G - v^ mean(G v^) is -v^ G v^, of 0.1, 2 and 64
+    vh = 2 * rho
+    for part, G in ((g.dx[:-3], 0.1), (g.dx[-3:], 64.0)):
+        G = float(torch.tensor(G).bfloat16())
+        d = -rho * vh * G * vh
+        # 4.5 u of v^ twice, 2.5 u of rho, three products, the sums before them
+        tol = torch.finfo(torch.bfloat16).eps / 2 * abs(d) + 16 * U * (abs(d) + 2 * abs(G))
+        assert (part.double() - d).abs().max().item() <= tol
